@@ -76,10 +76,9 @@ __device__ unsigned long long g_fwd_stamps[32];
 // delivers ~33 B/clk per CU (the same bound as the GEMM's operand delivery), and a wave's DMA instruction costs it ~80 issue cycles.
 // kWaves = 4: 128 queries, two workgroups per CU: the shapes with at most 128 queries (decoder self- and cross-attention).
 // kBits (dropout only): every keep decision also goes to AttnArgs::keep_bits for the backward (attn_common.h keep_bits_*).  The compare that
-// feeds the select IS the word the backward wants (a 64-bit lane mask in a scalar register pair), so it leaves by a scalar store:
-// s_store_dwordx4 of the two compares of a finish pair (gfx950 executes scalar stores -- tools/probe/probe_sstore.hip checks that and prices
-// one at ~7 instruction slots of its wave; the dirty lines leave the scalar cache at s_dcache_wb, before the wave ends).
-typedef unsigned u32x4s __attribute__((ext_vector_type(4)));
+// feeds the select IS the word the backward wants (a 64-bit lane mask in a scalar register pair): its two halves are written into lanes of one
+// register (v_writelane_b32), which leaves with a block's 32 words as one 128-byte vector store.
+__device__ unsigned write_lane(unsigned value, unsigned lane, unsigned old) __asm("llvm.amdgcn.writelane.i32");      // (clang has no builtin of that name)
 template <bool kDrop, int kWaves, bool kBits = false>
 __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(AttnArgs a, int n_items) {
   static_assert(kDrop || !kBits, "keep bits exist with dropout only");
@@ -112,7 +111,7 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(Attn
   int b, head, qi, klen;
   const unsigned short *kg, *vg;
   unsigned pb2;
-  const unsigned* bits_row = nullptr;      // kBits: keep words of (this item's head, this wave's 32-query slice, key block 0)
+  unsigned* bits_row = nullptr;            // kBits: keep words of (this item's head, this wave's 32-query slice, key block 0)
   auto set_item = [&](const Item& it) __attribute__((always_inline)) {
     b = it.b; head = it.head;
     qi = it.q0 + wave * 32 + r;
@@ -240,7 +239,8 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(Attn
   };
   // finish(g), pair s: two probabilities (left in place of the scores: phase B adds them up, it has the issue slots), dropout, one packed
   // bf16 pair of the P^T operand
-  auto finish_pair = [&](f32x16& st, int s, const unsigned* bits_blk) __attribute__((always_inline)) {      // bits_blk: the block's 32 keep words (kBits)
+  unsigned kwords;                     // kBits: the block's keep words, word w in lane w
+  auto finish_pair = [&](f32x16& st, int s) __attribute__((always_inline)) {
     float p0 = __builtin_amdgcn_exp2f(fmaf(st[2 * s], sl2, mneg)), p1 = __builtin_amdgcn_exp2f(fmaf(st[2 * s + 1], sl2, mneg));
     st[2 * s] = p0;
     st[2 * s + 1] = p1;
@@ -250,12 +250,22 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(Attn
       p1 = k1 ? p1 : 0.f;
       if (kBits) {                           // registers 2 s, 2 s + 1 of the block: words 4 s .. 4 s + 3
         const unsigned long long m0 = __builtin_amdgcn_ballot_w64(k0), m1 = __builtin_amdgcn_ballot_w64(k1);
-        const u32x4s w = {static_cast<unsigned>(m0), static_cast<unsigned>(m0 >> 32), static_cast<unsigned>(m1), static_cast<unsigned>(m1 >> 32)};
-        asm volatile("s_store_dwordx4 %0, %1, %2" :: "s"(w), "s"(bits_blk), "i"(16 * s));
+        if (s == 0) kwords = 0;              // (nothing of the block before it is carried)
+        kwords = write_lane(static_cast<unsigned>(m0), 4 * s, kwords);
+        kwords = write_lane(static_cast<unsigned>(m0 >> 32), 4 * s + 1, kwords);
+        kwords = write_lane(static_cast<unsigned>(m1), 4 * s + 2, kwords);
+        kwords = write_lane(static_cast<unsigned>(m1 >> 32), 4 * s + 3, kwords);
       }
     }
     pf[s >> 2].u[s & 3] = pack2_c(p0, p1);
     pin(pf[s >> 2].u[s & 3]);
+  };
+  auto store_words = [&](int kblk) __attribute__((always_inline)) {      // of 32-key block kblk, once its eight pairs are finished
+    if (kBits) {
+      unsigned ln = tid & 63;
+      asm volatile("" : "+v"(ln));         // (formed at the use: see dma_piece_of)
+      if (ln < 32) bits_row[kblk * 32 + ln] = kwords;
+    }
   };
   unsigned long long grow = 0;         // lanes whose block maximum exceeds the running one by more than kRescaleThr (taken inside phase B)
   auto rescale = [&]() __attribute__((always_inline)) {               // lazy: only when some row's maximum rose by more than kRescaleThr
@@ -284,17 +294,17 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(Attn
   // when no barrier lies between): the LDS round trip is not at the head of the MFMA chain.
   bf16x8 kf[8], vpre[4];
   auto phase_a = [&](f32x16& sn, int koff_, f32x16& sc, int vnext, int kblk) __attribute__((always_inline)) {      // vnext: LDS offset of the next phase B's V rows, -1: behind a barrier; kblk: 32-key block index of sc
-    const unsigned* bits_blk = kBits ? bits_row + kblk * 32 : nullptr;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sn[i] = 0.f;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       if (s < 4) kf[s + 4] = k_frag(s + 4, koff_);
       if (s >= 6 && vnext >= 0) { vpre[2 * (s - 6)] = v_frag(2 * (s - 6), vnext); vpre[2 * (s - 6) + 1] = v_frag(2 * (s - 6) + 1, vnext); }
-      finish_pair(sc, s, bits_blk);
+      finish_pair(sc, s);
       sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], qf[s], sn, 0, 0, 0);
       ADT_FENCE();
     }
+    store_words(kblk);
   };
   // ---- phase B: O^T += V(32 rows at LDS byte offset voff_)^T P^T   ||   row maximum of the block whose raw scores are in sn, its hashes
   // (a tile that needs the per-element mask gets it in a pass of its own in front of the phase: one tile in sixteen in the encoder)
@@ -382,9 +392,9 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(Attn
   // the last tile: no later tile to fetch or to start, and no second block when at most 32 of its keys exist (986 keys: block 31 of 32).
   // Run-time buffer offsets (an add per LDS read), once per workgroup.
   auto finish_only = [&](f32x16& sc, int kblk) __attribute__((always_inline)) {
-    const unsigned* bits_blk = kBits ? bits_row + kblk * 32 : nullptr;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) finish_pair(sc, s, bits_blk);
+    for (int s = 0; s < 8; ++s) finish_pair(sc, s);
+    store_words(kblk);
   };
   auto last_tile = [&](int t) __attribute__((always_inline)) {
     int kK = (t & 1) * 2 * kAttnTileBytes;
@@ -451,7 +461,6 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(Attn
     item = next_id;
     set_item(nxt);
   }
-  if (kBits) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::: "memory");      // the keep words leave the scalar cache
 }
 
 int launch_attn_fwd2(const AttnArgs& a, hipStream_t st) {

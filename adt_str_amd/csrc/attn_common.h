@@ -228,7 +228,7 @@ struct AttnArgs {
 // 64-bit lane mask, exactly { bits 0..31: queries 0..31 of the wave's slice for key acc_row(i, 0); bits 32..63: the same queries for key
 // acc_row(i, 1) } -- one 32-bit word per key with a bit per query, which is what the backward (KEY on the lane) wants in a vector register.
 // Layout: [batch * head][32-query slice][32-key block][32 words], word 2 i + h <-> key acc_row(i, h) of the block; the forward stores the
-// compare results from its scalar registers (s_store_dwordx4: 16 bytes = registers 2 s, 2 s + 1), the backward's lane for key r loads word
+// compare results of a block as one 128-byte vector store (lane = word), the backward's lane for key r loads word
 // keep_bits_word(r) and tests bit q.  Slices / blocks are padded to whole 256s of queries / keys so that neither kernel needs a bounds test;
 // blocks past the key range and slices past the query range hold garbage that is never used (their probabilities are zero).
 __host__ __device__ __forceinline__ int keep_bits_word(int key) { return 2 * ((key & 3) + 4 * (key >> 3)) + ((key >> 2) & 1); }
