@@ -506,10 +506,9 @@ __global__ __launch_bounds__(kFbThreads, 1) void attn_bwd_fused_kernel(FusedArgs
     // kDrop == 2: wb = the lane's keep word of the block, shifted right by 4 h (so that the bit of accumulator register i sits at
     // position acc_row(i, 0)); v_bfe_i32 spreads the bit over the register, an AND with 1 / (1 - p) gives the keep scale
     unsigned wb0 = 0, wb1 = 0;
-    // Two elements per call, on register PAIRS (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32: accumulator registers 2 m, 2 m + 1 are an
-    // aligned pair, and so are their row constants): one wave per SIMD issues a vector instruction every ~5 cycles whatever it is
-    // (tools/probe/probe_mfma_valu), so what counts is the NUMBER of instructions beside the products -- per pair 7 without dropout
-    // (10 before), 11 with the keep bits.  P arrives scaled by 1 / (1 - p) (folded into the chain's initial accumulator nl), the keep decision is an AND (bits) or a
+    // Two elements per call, written on register PAIRS (accumulator registers 2 m, 2 m + 1 and their row constants; the build keeps the
+    // arithmetic itself scalar, see the Makefile): one wave per SIMD issues a vector instruction every ~5 cycles whatever it is
+    // (tools/probe/probe_mfma_valu), so what counts is the NUMBER of instructions beside the products.  P arrives scaled by 1 / (1 - p) (folded into the chain's initial accumulator nl), the keep decision is an AND (bits) or a
     // select (hash) on it, and dS = P_dropped dP + P' nd' with nd' = -delta (1 - p) -- no separate keep-scale product.
     auto arith_pair = [&](int m, const f32x16& st, const f32x16& dp, const uint64_t (&km)[16], unsigned wb, float pad2, float kval, int qrel,
                           unsigned (&hp)[8], unsigned (&hs)[8]) {

@@ -405,8 +405,8 @@ __global__ __launch_bounds__(kFbThreads, 1) void attn_bwd_fused8_kernel(FusedArg
     // kDrop == 2: wb = the lane's keep word of the block, shifted right by 4 h (so that the bit of accumulator register i sits at
     // position acc_row(i, 0)); v_bfe_i32 spreads the bit over the register, an AND with 1 / (1 - p) gives the keep scale
     unsigned wb = 0;
-    // Two elements per call, on register PAIRS (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32: accumulator registers 2 m, 2 m + 1 are an
-    // aligned pair, and so are their row constants); attention_bwd_fused.hip has the derivation.
+    // Two elements per call, written on register PAIRS (accumulator registers 2 m, 2 m + 1 and their row constants); attention_bwd_fused.hip has
+    // the derivation.
     auto arith_pair = [&](int m) {
       const int i0 = 2 * m, g = i0 >> 2, c0 = i0 & 3;
       const f32x2 s2 = {st[i0], st[i0 + 1]}, d2 = {dp[i0], dp[i0 + 1]};

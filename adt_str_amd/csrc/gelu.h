@@ -15,7 +15,7 @@ __device__ __forceinline__ float gauss_cdf(float x, float& e) {
 }
 __device__ __forceinline__ float gelu_erf(float x) { float e; return x * gauss_cdf(x, e); }
 __device__ __forceinline__ float gelu_erf_grad(float x) { float e; const float c = gauss_cdf(x, e); return fmaf(x * 0.3989422804014327f, e, c); }
-// The same arithmetic on register pairs (v_pk_fma_f32 / v_pk_mul_f32: two elements per instruction; only rcp and exp stay scalar):
+// The same arithmetic on pairs of elements:
 // hq = 0.5 erfc(|x| / sqrt 2) and e = exp(-x^2 / 2) of both elements.  GELU is then max(x, 0) - |x| hq on either side of 0.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 half_erfc2(f32x2 x, f32x2 ax, f32x2& e) {

@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256) void htsat_patch_embed_tok_kernel(const float*
 #pragma unroll
   for (int o = 0; o < C; ++o) {
     float acc = bias[o];
-    // (asm: left to the compiler, channel pairs are SLP-packed into v_pk_fma_f32 whose weight pairs -- 16 floats apart in memory --
+    // (asm: left to the compiler, a compiler that packs channel pairs uses weight pairs -- 16 floats apart in memory --
     // are then assembled with a v_readlane and two s_mov each: more instructions than the FMAs themselves)
 #pragma unroll
     for (int e = 0; e < 16; ++e) asm("v_fmac_f32 %0, %1, %2" : "+v"(acc) : "s"(w[o * 16 + e]), "v"(px[e]));

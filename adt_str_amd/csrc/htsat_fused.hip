@@ -785,8 +785,7 @@ __device__ __forceinline__ unsigned pack2_c(float lo, float hi) {
   typedef float f32x2_ __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2_{lo, hi}, bf16x2_));
 }
-// p = 2^(s - mx) over a wave's 2 x 16 scores, and their sum: the subtraction and the sums on register pairs (v_pk_add_f32: half the
-// instructions), four independent partial sums instead of one chain of 32 dependent adds
+// p = 2^(s - mx) over a wave's 2 x 16 scores, and their sum: the subtraction and the sums in pairs, four independent partial sums instead of one chain of 32 dependent adds
 __device__ __forceinline__ float softmax_exp_sum(f32x16 (&st)[2], float mx) {
   const f32x2 m2 = {mx, mx};
   f32x2 ps[2][2] = {{{0.f, 0.f}, {0.f, 0.f}}, {{0.f, 0.f}, {0.f, 0.f}}};
@@ -984,7 +983,7 @@ __global__ __launch_bounds__(256, 2) void htsat_attn_kernel(AtArgs a) {
       for (int g = 0; g < 4; ++g) {
         const float bb[4] = {rbv[kt][g].x, rbv[kt][g].y, rbv[kt][g].z, rbv[kt][g].w};
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {                             // log2 domain: the bias table comes pre-multiplied by log2 e (pairs: v_pk_fma_f32)
+        for (int e = 0; e < 4; e += 2) {                             // log2 domain: the bias table comes pre-multiplied by log2 e
           const f32x2 v = f32x2{st[kt][4 * g + e], st[kt][4 * g + e + 1]} * sl2 + f32x2{bb[e], bb[e + 1]};
           st[kt][4 * g + e] = v[0]; st[kt][4 * g + e + 1] = v[1];
           mx = fmaxf(mx, fmaxf(v[0], v[1]));
@@ -1349,7 +1348,7 @@ __global__ __launch_bounds__(256, C == 192 ? 2 : 1) void htsat_attn_big_kernel(A
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {                               // log2 domain: the bias table comes pre-multiplied by log2 e (pairs: v_pk_fma_f32)
+        for (int e = 0; e < 4; e += 2) {                               // log2 domain: the bias table comes pre-multiplied by log2 e
           const f32x2 v = f32x2{st[kt][4 * g + e], st[kt][4 * g + e + 1]} * sl2 + f32x2{rbv[g][e], rbv[g][e + 1]};
           st[kt][4 * g + e] = v[0]; st[kt][4 * g + e + 1] = v[1];
           mx = fmaxf(mx, fmaxf(v[0], v[1]));

@@ -21,12 +21,10 @@ namespace adt {
 constexpr int kNfft = 2048;
 
 // Complex arithmetic.  On the device a complex number is a register PAIR (ext_vector_type(2)) and every operation below is written as
-// whole-pair arithmetic the compiler turns into ONE packed instruction each (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32 with op_sel
-// swizzles): a rotation by -i is a swapped operand times the constant pair (1, -1) inside an FMA, a complex product is a packed
-// multiply and a packed FMA (plus one packed multiply for i b when b is not a compile-time constant).  Written element by element
-// (the struct form the host emulator keeps) the same kernels carried ~200 v_mov / v_pk_mov register shuffles per frame -- a sixth of
-// their instructions -- because the compiler folds a swizzle into a packed operand but not a swizzle with a per-element sign
-// (round 5: K1 and K9 are bound by vector instruction issue, so instructions are what counts).
+// whole-pair arithmetic: a rotation by -i is a swapped operand times the constant pair (1, -1) inside an FMA, a complex product is a
+// multiply and an FMA of pairs.  K1 and K9 are bound by vector instruction issue; the build takes the pairs apart into scalar
+// instructions (see the Makefile), which measured 8 % faster here than packed ones with their swizzles and register moves
+// (398 k -> 434 k clips/s of 10 s, one chip, same run).
 #if defined(__HIP_DEVICE_COMPILE__)
 typedef float cf __attribute__((ext_vector_type(2)));
 ADT_HD cf cswap_(cf a) { return __builtin_shufflevector(a, a, 1, 0); }
