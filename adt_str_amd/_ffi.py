@@ -18,7 +18,7 @@ if os.environ.get("ADT_LIB_PATH"):          # said on stderr so that a bench lin
 _lock = threading.Lock()
 _lib = None
 
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 i32, i64, f32, ptr = C.c_int32, C.c_int64, C.c_float, C.c_void_p
 
@@ -51,6 +51,12 @@ class AttnDesc(C.Structure):
                 ("ldv", C.c_int64), ("ldo", C.c_int64), ("scale", C.c_float), ("mask_value", C.c_float),
                 ("key_len", C.c_void_p), ("drop", Dropout), ("dq_colsum", C.c_void_p), ("dk_colsum", C.c_void_p),
                 ("dv_colsum", C.c_void_p), ("keep_bits", C.c_void_p), ("f32_products", C.c_int32)]
+
+
+class AttnKv4Desc(C.Structure):
+    """struct adt_attn_kv4_desc (include/adt_hip.h)."""
+    _fields_ = [("batch", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("q_len", C.c_int32),
+                ("capacity", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float), ("ldq", C.c_int64), ("ldo", C.c_int64), ("key_len", C.c_void_p)]
 
 
 class AffWeights(C.Structure):
@@ -108,6 +114,13 @@ SIGNATURES = {
     "adt_layernorm_bwd_f32": [ptr, i64, ptr, i64, ptr, ptr, ptr, ptr, ptr, i64, ptr, ptr, ptr, i64, i64, ptr, ptr, ptr, C.c_size_t, ptr],
     "adt_cross_entropy_f32": [ptr, i64, ptr, i64, i64, i64, ptr, ptr, i64, ptr, C.c_size_t, ptr],
     "adt_embed_bwd_operands_f32": [ptr, ptr, f32, ptr, i64, ptr, i64, i64, i64, ptr, ptr],
+    "adt_quant_rows_i8": [ptr, i32, i64, i64, i64, ptr, i64, ptr, ptr],
+    "adt_gemm_i8": [i64, i64, i64, ptr, i64, ptr, ptr, i64, ptr, ptr, i64, ptr, ptr],
+    "adt_kv4_bytes": [i64, i32, i32, i64],
+    "adt_kv4_append": [ptr, i64, i32, i32, i64, ptr, i64, ptr, i64, i64, ptr, ptr, ptr],
+    "adt_kv4_read": [ptr, i64, i32, i32, i64, ptr, i64, ptr, i64, i32, i64, ptr, ptr, ptr],
+    "adt_attn_kv4_workspace_bytes": [ptr],
+    "adt_attn_kv4": [ptr, ptr, ptr, ptr, ptr, ptr, C.c_size_t, ptr],
     "adt_cast_bf16": [ptr, ptr, ptr, i64, i64, ptr],
     "adt_cast_bf16_batched": [ptr, i32, i32, ptr],
     "adt_grad_norm_workspace_bytes": [],
@@ -140,7 +153,7 @@ _RESTYPES.update({n: C.c_size_t for n in ("adt_mix_workspace_bytes", "adt_gemm_w
                                           "adt_cross_entropy_workspace_bytes", "adt_grad_norm_workspace_bytes",
                                           "adt_htsat_fusion_embed_workspace_bytes",
                                           "adt_attn_bwd_f32_workspace_bytes", "adt_colsum_f32_workspace_bytes", "adt_gemm_f32_workspace_bytes",
-                                          "adt_gemm_bf16x3_workspace_bytes")})
+                                          "adt_gemm_bf16x3_workspace_bytes", "adt_kv4_bytes", "adt_attn_kv4_workspace_bytes")})
 
 
 class AdtError(RuntimeError):

@@ -638,3 +638,180 @@ def check_attn_bwd() -> None:
     if n > 0:
         raise RuntimeError(f"adt_attn_bwd: {n} wave(s) of the one-kernel attention backward gave up waiting for a dQ tile in an earlier "
                            "launch (its dQ was incomplete); the step's gradients are not to be trusted")
+
+
+# ---- serving in few bits: 8-bit-integer linear layers (K16) ------------------------------------------------------------------------
+class _on_device:
+    """The launches inside go to the current stream of the tensors' own device, whichever device is current; all tensors must share it."""
+    __slots__ = ("index", "back")
+
+    def __init__(self, *tensors):
+        dev = None
+        for t in tensors:
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise RuntimeError("adt_str_amd kernels take GPU tensors only (there is no CPU path)")
+            i = t.get_device()
+            if dev is None:
+                dev = i
+            elif i != dev:
+                raise RuntimeError(f"tensors of one call lie on different devices ({dev} and {i})")
+        self.index = dev
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, exc_type, exc, tb):
+        if self.back != self.index:
+            torch.cuda.set_device(self.back)
+        return False
+
+
+def quant_rows_i8(x: torch.Tensor):
+    """``x [M, K]`` bf16 or fp32 (row-strided views allowed) -> ``(q int8 [M, K16], scale fp32 [M])``, ``K16`` = K rounded up to 16 with zero
+    columns: one scale per row, ``scale = max|x| / 127``, ``q`` the integer nearest to ``127 x / max|x|`` (ties to even).  A row with an infinity
+    or a NaN gets the scale NaN.  Serves activations (scale per token) and weights ``[N, K]`` (scale per output channel) alike."""
+    assert x.dtype in (torch.bfloat16, torch.float32) and x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1)
+    M, K = x.shape
+    with _on_device(x) as stream:
+        q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+        scale = torch.empty(M, dtype=torch.float32, device=x.device)
+        _ffi.call("adt_quant_rows_i8", x.data_ptr() if M else 16, int(x.dtype == torch.float32), x.stride(0) if M > 1 else max(x.stride(0), K), M, K,
+                  q.data_ptr() if M else 16, q.shape[1], scale.data_ptr() if M else 16, stream)
+    return q, scale
+
+
+def _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux):
+    assert act in (0, 1, 2)
+    assert out.shape == (M, N) and out.dtype in (torch.bfloat16, torch.float32) and (N <= 1 or out.stride(1) == 1)
+    ep = _ffi.GemmEpilogue()
+    ep.alpha, ep.act, ep.out_fp32 = 1.0, act, int(out.dtype == torch.float32)
+    if bias is not None:
+        assert bias.dtype == torch.float32 and bias.numel() == N and bias.is_contiguous()
+        ep.bias = bias.data_ptr()
+    if residual is not None:
+        assert residual.dtype == torch.float32 and residual.dim() == 2 and residual.shape[1] == N and (N == 1 or residual.stride(1) == 1)
+        assert res_row_mod >= 0 and residual.shape[0] >= (res_row_mod or M)
+        ep.residual, ep.ld_res, ep.res_row_mod = residual.data_ptr(), max(residual.stride(0), N), res_row_mod
+    if aux is not None:
+        assert out.dtype == torch.float32 and aux.dtype == torch.bfloat16 and aux.shape == (M, N) and (N == 1 or aux.stride(1) == 1)
+        ep.aux_bf16_out, ep.ld_aux = aux.data_ptr(), max(aux.stride(0), N)
+    return ep
+
+
+def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+            out_dtype=torch.bfloat16, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, res_row_mod: int = 0,
+            act: int = 0, aux_bf16_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act((a [M, K] @ b [N, K].T) * a_scale[:, None] * b_scale + bias) + residual`` with int8 operands and exact integer sums (``adt_gemm_i8``):
+    the inference epilogue of :func:`gemm`.  ``K`` is a multiple of 16 (``quant_rows_i8`` pads), at most 131072."""
+    assert a.dtype == torch.int8 and b.dtype == torch.int8 and a.dim() == 2 and b.dim() == 2 and a.shape[1] == b.shape[1]
+    (M, K), N = a.shape, b.shape[0]
+    assert K > 0 and K % 16 == 0 and a.stride(1) == 1 and b.stride(1) == 1
+    for s, n in ((a_scale, M), (b_scale, N)):
+        assert s.dtype == torch.float32 and s.dim() == 1 and s.numel() == n and s.is_contiguous()
+    with _on_device(a, a_scale, b, b_scale, out, bias, residual, aux_bf16_out) as stream:
+        if out is None:
+            out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+        ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
+        if M and N:
+            _ffi.call("adt_gemm_i8", M, N, K, a.data_ptr(), max(a.stride(0), K), a_scale.data_ptr(), b.data_ptr(), max(b.stride(0), K), b_scale.data_ptr(),
+                      out.data_ptr(), max(out.stride(0), N), C.byref(ep), stream)
+    return out
+
+
+def linear_i8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, **kw) -> torch.Tensor:
+    """``x [M, K]`` (bf16 / fp32) through a linear layer whose weights are int8 with one scale per output channel (``w8, w_scale =
+    quant_rows_i8(weight)``): the rows are quantised (``quant_rows_i8``) and multiplied (``gemm_i8``, whose keyword arguments this takes)."""
+    assert x.dim() == 2 and w8.dim() == 2 and w8.shape[1] == (x.shape[1] + 15) // 16 * 16, (x.shape, w8.shape)
+    q, scale = quant_rows_i8(x)
+    return gemm_i8(q, scale, w8, w_scale, **kw)
+
+
+# ---- serving in few bits: the 4-bit K/V cache (K17) --------------------------------------------------------------------------------
+class KV4Cache:
+    """K and V rows of ``batch`` sequences with up to ``capacity`` positions each, ``kv_heads`` heads of ``head_dim`` (64 or 128) channels, in 4 bits
+    per value with a bf16 scale and minimum per 64 channels: 72 bytes per row of 128 channels (bf16: 256).  The memory is not cleared; the
+    caller keeps the lengths and names them on every call (``adt_kv4_*``)."""
+    __slots__ = ("batch", "capacity", "kv_heads", "head_dim", "data")
+
+    def __init__(self, batch: int, capacity: int, kv_heads: int, head_dim: int, device="cuda"):
+        if head_dim not in (64, 128):
+            raise NotImplementedError("the 4-bit cache is built for heads of 64 or 128 channels")
+        if batch < 0 or capacity <= 0 or kv_heads <= 0:
+            raise ValueError("a cache has a capacity and heads")
+        self.batch, self.capacity, self.kv_heads, self.head_dim = int(batch), int(capacity), int(kv_heads), int(head_dim)
+        self.data = torch.empty(_ffi.load().adt_kv4_bytes(batch, kv_heads, head_dim, capacity), dtype=torch.uint8, device=device)
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel()
+
+
+def _kv4_rows(cache, end, count, k, v, n):
+    for t in (end, count):
+        assert t is None or (t.dtype == torch.int32 and t.dim() == 1 and t.numel() == cache.batch and t.is_contiguous())
+    width = cache.kv_heads * cache.head_dim
+    for t in (k, v):
+        assert t.dim() == 2 and t.shape == (cache.batch * n, width) and t.stride(1) == 1, (t.shape, cache.batch, n, width)
+    return width
+
+
+def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, end: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None) -> None:
+    """Quantise K and V rows into the cache.  ``k``, ``v``: bf16 ``[batch * n, kv_heads * head_dim]`` (row-strided views allowed), n rows per
+    sequence.  Row i < ``count[b]`` (int32, default n) goes to position ``end[b] - count[b] + i`` (``end`` int32: the sequence's length after
+    the call, the ``key_len`` of :func:`attn_kv4`; default the capacity); the other rows are left out, as are positions outside the cache."""
+    assert k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16 and k.shape == v.shape
+    if cache.batch == 0 or k.shape[0] == 0:
+        return
+    assert k.shape[0] % cache.batch == 0, (k.shape, cache.batch)
+    n = k.shape[0] // cache.batch
+    width = _kv4_rows(cache, end, count, k, v, n)
+    with _on_device(cache.data, k, v, end, count) as stream:
+        _ffi.call("adt_kv4_append", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity, k.data_ptr(), max(k.stride(0), width),
+                  v.data_ptr(), max(v.stride(0), width), n, end.data_ptr() if end is not None else None, count.data_ptr() if count is not None else None, stream)
+
+
+def kv4_read(cache: KV4Cache, end: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None, n: Optional[int] = None, out_dtype=torch.bfloat16):
+    """The rows that ``kv4_append(cache, k, v, end, count)`` with n rows per sequence would write, as the values the cache holds ->
+    ``(k, v) [batch * n, kv_heads * head_dim]`` in bf16 or fp32 (default: the whole capacity); rows i >= ``count[b]`` are zeros."""
+    assert out_dtype in (torch.bfloat16, torch.float32)
+    n = cache.capacity if n is None else int(n)
+    assert n >= 0
+    width = cache.kv_heads * cache.head_dim
+    with _on_device(cache.data, end, count) as stream:
+        k, v = (torch.empty((cache.batch * n, width), dtype=out_dtype, device=cache.data.device) for _ in range(2))
+        if cache.batch and n:
+            _kv4_rows(cache, end, count, k, v, n)
+            _ffi.call("adt_kv4_read", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity, k.data_ptr(), width, v.data_ptr(), width,
+                      int(out_dtype == torch.float32), n, end.data_ptr() if end is not None else None, count.data_ptr() if count is not None else None, stream)
+    return k, v
+
+
+def attn_kv4(q: torch.Tensor, cache: KV4Cache, key_len: Optional[torch.Tensor] = None, *, heads: int, scale: float, q_len: int = 1, causal: bool = False,
+             out: Optional[torch.Tensor] = None, want_lse: bool = False):
+    """Attention of ``q [batch * q_len, >= heads * head_dim]`` (bf16, row-strided views allowed) over the cache's first ``key_len[b]`` positions
+    (int32, default the capacity) -> ``o [batch * q_len, heads * head_dim]`` bf16, with ``want_lse`` also the log-sum-exp rows fp32
+    ``[batch, heads, q_len]``.  ``heads`` is a multiple of the cache's ``kv_heads`` (grouped heads).  ``causal``: the queries are the sequence's
+    last ``q_len`` positions, query i sees ``key_len[b] - (q_len - 1 - i)`` of them.  A query that sees none gets zeros (lse -inf)."""
+    width = heads * cache.head_dim
+    rows = cache.batch * q_len
+    assert q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q_len > 0 and heads > 0 and heads % cache.kv_heads == 0
+    assert q.shape[0] == rows and q.shape[1] >= width, (q.shape, rows, width)
+    assert key_len is None or (key_len.dtype == torch.int32 and key_len.dim() == 1 and key_len.numel() == cache.batch and key_len.is_contiguous())
+    with _on_device(q, cache.data, key_len, out) as stream:
+        if out is None:
+            out = torch.empty((rows, width), dtype=torch.bfloat16, device=q.device)
+        assert out.dtype == torch.bfloat16 and out.shape == (rows, width) and out.stride(1) == 1
+        lse = torch.empty((cache.batch, heads, q_len), dtype=torch.float32, device=q.device) if want_lse else None
+        if rows:
+            d = _ffi.AttnKv4Desc(cache.batch, heads, cache.kv_heads, cache.head_dim, q_len, cache.capacity, int(causal), float(scale),
+                                 max(q.stride(0), width), max(out.stride(0), width), key_len.data_ptr() if key_len is not None else None)
+            nb = _ffi.load().adt_attn_kv4_workspace_bytes(C.byref(d))
+            ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None       # (from the allocator: a captured call gets its graph's own)
+            _ffi.call("adt_attn_kv4", C.byref(d), q.data_ptr(), cache.data.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
+                      ws.data_ptr() if nb else None, nb, stream)
+    return (out, lse) if want_lse else out

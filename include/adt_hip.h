@@ -40,7 +40,7 @@ extern "C" {
  * backward entry points regenerate them from the same (p, key).  p == 0 or a null pointer: off. */
 typedef struct adt_dropout { float p; uint32_t key; } adt_dropout;
 
-/* ABI version (18): bumped whenever a signature below changes or entries are added. */
+/* ABI version (20): bumped whenever a signature below changes or entries are added. */
 int adt_version(void);
 
 /* Message of the last failing call on this thread ("" if none). */
@@ -452,6 +452,56 @@ size_t adt_gemm_bf16x3_workspace_bytes(int32_t trans, int64_t M, int64_t N, int6
 int adt_gemm_bf16x3(int32_t trans, int64_t M, int64_t N, int64_t K, const void* A2, int64_t lda, int64_t a_lo,
                     const void* B2, int64_t ldb, int64_t b_lo, float* C, int64_t ldc, const adt_gemm_epilogue* ep,
                     void* ws, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * K16  serving in few bits: products in 8-bit integers (adt_str_amd/csrc/gemm_i8.hip)
+ *
+ * The inference form of the path's nn.Linear layers (reference model.py:111,118-127,157,159-168,224): activations with one scale per row
+ * (token), weights with one scale per output channel, exact int32 sums.
+ *
+ *   adt_quant_rows_i8   x [M, K] bf16 (x_fp32 != 0: fp32), any K >= 1, row stride ldx in elements ->
+ *                       a_m = max(max_k |x_mk|, 2^-100);  q_mk = the integer nearest to 127 x_mk / a_m, ties to even;  scale_m = a_m / 127
+ *                       q int8 [M, ldq], columns [K, K rounded up to 16) zero; ldq a multiple of 16, rows 16-byte aligned.  A row with an
+ *                       infinity or a NaN: scale NaN, codes 0, so that whatever is computed from it is NaN.
+ *   adt_gemm_i8         C[M, N] = act(A[M, K] . B[N, K]^T * a_scale[m] * b_scale[n] + bias[n]) + residual, int8 operands, fp32 scales.
+ *                       K a multiple of 16 up to 131072 (pad with zeros), operand rows 16-byte aligned; any M and N >= 0.
+ *                       ep: bias, act, residual (+ res_row_mod), out_fp32, aux_bf16_out (with an fp32 C), as adt_gemm_bf16; alpha must be 1;
+ *                       the training fields must be null / 0 (ADT_EINVAL). */
+int adt_quant_rows_i8(const void* x, int32_t x_fp32, int64_t ldx, int64_t M, int64_t K, void* q, int64_t ldq, float* scale, void* stream);
+int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const float* a_scale, const void* B, int64_t ldb,
+                const float* b_scale, void* C, int64_t ldc, const adt_gemm_epilogue* ep, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * K17  serving in few bits: a K/V cache held in 4 bits (adt_str_amd/csrc/kv4.hip)
+ *
+ * The caches of the KV-cached greedy decode (reference model.py:260-324 re-runs the decoder instead) at 72 bytes per K or V row of 128
+ * channels instead of 256.  Every 64 channels of a row share a bf16 scale s and a bf16 minimum m; a value is c s + m with a code c in 0 .. 15:
+ *   m = min x,  s = bf16(max((max x - m) / 15, 2^-100)),  c = min(15, the integer nearest to (x - m) / s, ties to even)
+ * A group with an infinity or a NaN, or whose range exceeds fp32, stands for NaNs.
+ *
+ *   adt_kv4_bytes    size of a cache of `capacity` positions per sequence (head_dim 64 or 128); opaque device memory, 16-byte aligned.  It
+ *                    need not be cleared: only rows below the lengths that a call names are read.
+ *   adt_kv4_append   k, v: bf16 rows, n per sequence (row b * n + i, head h at columns h * head_dim), row strides in elements.  Row i < count[b]
+ *                    goes to position end[b] - count[b] + i; count null: n rows, end null: capacity.  Rows i >= count[b], and rows whose position
+ *                    lies outside [0, capacity), are left out; every other position keeps what it held.
+ *   adt_kv4_read     the same rows back as the values they stand for, bf16 or fp32 (out_fp32) [batch * n, ld]; rows the cache does not have: zeros.
+ *   adt_attn_kv4     o = softmax(q k^T * scale) v over the positions below key_len[b] (null: capacity), q and o bf16 [batch * q_len, >= heads *
+ *                    head_dim].  heads is a multiple of kv_heads: query heads g * kv_head .. + g - 1 read K/V head kv_head (g = heads / kv_heads).
+ *                    causal: query i sees the positions below key_len[b] - (q_len - 1 - i), that is, the queries are the sequence's last
+ *                    positions.  A query that sees no position gets zeros (lse -inf).  lse: optional fp32 [batch, heads, q_len]. */
+size_t adt_kv4_bytes(int64_t batch, int32_t kv_heads, int32_t head_dim, int64_t capacity);
+int adt_kv4_append(void* cache, int64_t batch, int32_t kv_heads, int32_t head_dim, int64_t capacity, const void* k, int64_t ldk, const void* v,
+                   int64_t ldv, int64_t n, const int32_t* end, const int32_t* count, void* stream);
+int adt_kv4_read(const void* cache, int64_t batch, int32_t kv_heads, int32_t head_dim, int64_t capacity, void* k, int64_t ldk, void* v, int64_t ldv,
+                 int32_t out_fp32, int64_t n, const int32_t* end, const int32_t* count, void* stream);
+typedef struct adt_attn_kv4_desc {
+  int32_t batch, heads, kv_heads, head_dim, q_len, capacity, causal;
+  float   scale;
+  int64_t ldq, ldo;
+  const int32_t* key_len;
+} adt_attn_kv4_desc;
+size_t adt_attn_kv4_workspace_bytes(const adt_attn_kv4_desc* d);
+int adt_attn_kv4(const adt_attn_kv4_desc* d, const void* q, const void* cache, void* o, float* lse, void* ws, size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Parameter plumbing for the bf16 compute path: fp32 master weight [rows, cols]
