@@ -32,7 +32,7 @@ from . import kernels as K
 from .frontend import ComputeMelSpectrogram
 
 F32, BF16 = torch.float32, torch.bfloat16
-PRECISIONS = ("bf16", "fp32", "bf16x3")
+PRECISIONS = ("bf16", "fp32", "bf16x3", "int8")
 
 
 class ADTModelConfig(PretrainedConfig):
@@ -114,6 +114,7 @@ class _Lin:
     def __init__(self, name: str, weight: nn.Parameter, bias: Optional[nn.Parameter]):
         self.name, self.weight, self.bias = name, weight, bias
         self.w16 = self.wt16 = None
+        self.w8 = self.w_scale = None                    # precision "int8": one scale per output channel
 
     def refresh(self):
         self.w16, self.wt16 = K.cast_bf16(self.weight.data.contiguous(), True, True)
@@ -128,7 +129,9 @@ class _Engine:
     ``"fp32"`` (the exact parity arm: fp32 activations end to end on the f32-input MFMA kernels of ``csrc/precise.hip``) or
     ``"bf16x3"`` (the fast parity arm: the same fp32 activations and the same kernels, every product taken as three bf16 MFMAs on
     hi / lo splits of the fp32 operands -- ~1e-5 relative per product instead of 6e-8, on the 16 x faster matrix pipe).  Both parity
-    arms meet BASELINE's "logits within 1e-3 rel-tol of the CPU reference".  Default from ``ADT_PRECISION``."""
+    arms meet BASELINE's "logits within 1e-3 rel-tol of the CPU reference".  ``"int8"`` is the bf16 path for inference with the linear layers of
+    the encoder and decoder stacks as 8-bit-integer products (one scale per token and output channel, exact integer sums; the mel
+    projection, the generator, attention and LayerNorm stay as they are); it has no backward pass.  Default from ``ADT_PRECISION``."""
 
     def __init__(self, model: "ADTModel", precision: Optional[str] = None):
         self.m = model
@@ -137,7 +140,8 @@ class _Engine:
         if precision not in PRECISIONS:
             raise ValueError(f"precision must be one of {PRECISIONS}, not {precision!r}")
         self.precision = precision
-        self.fp32 = precision != "bf16"                   # fp32 activations / operands (both parity arms)
+        self.int8 = precision == "int8"                   # inference: quantised linear layers, otherwise the bf16 path
+        self.fp32 = precision not in ("bf16", "int8")     # fp32 activations / operands (both parity arms)
         self.products = "bf16x3" if precision == "bf16x3" else "f32"     # how the fp32-operand kernels multiply (kernels.f32_products)
         self.adt = F32 if self.fp32 else BF16            # dtype of GEMM / attention operands and stored activations
         self.H, self.d, self.dh = cfg.nhead, cfg.nhead * cfg.d_query, cfg.d_query
@@ -235,6 +239,10 @@ class _Engine:
                         l.w16, l.wt16 = y, yt
                 self._cast_table.run()
             self._kv_cat = None                           # concatenated cross-attention K|V operands follow the weights
+            if self.int8:
+                for l in lins:
+                    if l is not self.proj and l is not self.gen:
+                        l.w8, l.w_scale = K.quant_rows_i8(l.weight.data.contiguous())
             self._versions = tuple(p._version for p in self.named.values()) + (ver[-1],)
 
     def _kv_operands(self):
@@ -265,13 +273,28 @@ class _Engine:
         """fp32 activation -> GEMM operand (a bf16 copy, or the tensor itself on the fp32 path)."""
         return x32 if self.fp32 else K.cast_bf16(x32)[0]
 
-    def _gemm_dual(self, a, w, **kw):
+    def _lin(self, x, lin: _Lin, lo=None, hi=None, **kw):
+        """Forward product with rows [lo, hi) of a layer's weight (+ the epilogue ``kw``).  ``x``: the operand, or in int8 mode also what
+        ``_quant`` made of it (an operand of several layers is quantised once)."""
+        part = (lambda t: t) if lo is None and hi is None else (lambda t: t[lo:hi])
+        bias = None if lin.b is None else part(lin.b)
+        if lin.w8 is None:
+            return K.gemm(x, part(lin.w16), bias=bias, **kw)
+        if kw.get("drop", 0) is None:                     # inference: no dropout site is on
+            kw = {k: v for k, v in kw.items() if k not in ("drop", "drop_after_residual")}
+        q, scale = x if isinstance(x, tuple) else K.quant_rows_i8(x)
+        return K.gemm_i8(q, scale, part(lin.w8), part(lin.w_scale), bias=bias, **kw)
+
+    def _quant(self, x):
+        return K.quant_rows_i8(x) if self.int8 else x
+
+    def _gemm_dual(self, a, lin: _Lin, **kw):
         """GEMM whose result is needed as the fp32 residual stream AND as the next GEMM's operand -> (x32, x16)."""
         if self.fp32:
-            x32 = K.gemm(a, w, **kw)
+            x32 = K.gemm(a, lin.w16, **kw)
             return x32, x32
-        x16 = torch.empty((a.shape[0], w.shape[0]), dtype=BF16, device=a.device)
-        return K.gemm(a, w, out_dtype=F32, aux_bf16_out=x16, **kw), x16
+        x16 = torch.empty((a.shape[0], lin.w16.shape[0]), dtype=BF16, device=a.device)
+        return self._lin(a, lin, out_dtype=F32, aux_bf16_out=x16, **kw), x16
 
     def _dgrad(self, dy, lin: _Lin, lo=None, hi=None, **kw):
         """Data gradient ``dy @ W[lo:hi]`` (bf16: NT GEMM against the transposed copy; fp32: NN GEMM against the master)."""
@@ -304,7 +327,7 @@ class _Engine:
     def _lean_ln(self) -> bool:
         """LayerNorms inside the layer stacks write only their bf16 output; the fp32 residual is rebuilt by the consuming GEMM's
         epilogue (bf16 path; ADT_NO_RES_LN=1 keeps the fp32 outputs, for A/B runs)."""
-        return not self.fp32 and not os.environ.get("ADT_NO_RES_LN")
+        return not self.fp32 and not self.int8 and not os.environ.get("ADT_NO_RES_LN")
 
     def _ln_bwd(self, *a, **kw):
         return K.layernorm_bwd(*a, branch_dtype=self.adt, **kw)
@@ -316,6 +339,13 @@ class _Engine:
         return K.embed_pe_fwd(tokens, emb, pe, scale, drop=drop)
 
     # ---- forward pieces -------------------------------------------------------------
+    def _ffn1(self, x, lin: _Lin, p):
+        """``(u, h)``: dropout(GELU(linear1(x))) and the factor its backward multiplies by (None in int8 mode)."""
+        if self.int8:
+            return None, self._lin(x, lin, act=1)
+        u = torch.empty((x.shape[0], lin.w16.shape[0]), dtype=self.adt, device=x.device)
+        return u, K.gemm(x, lin.w16, bias=lin.b, act=1, act_grad_out=u, drop=self.D(p + ".ffn"))
+
     def _encoder_fwd(self, src, save: Optional[list]):
         m, d, H = self.m, self.d, self.H
         mel = m.compute_spectrogram(src)                                   # K1: [B, S, n_mels] fp32
@@ -324,7 +354,7 @@ class _Engine:
         mel16 = self._operand(mel.view(M, n_mels))
         x0 = K.gemm(mel16, self.proj.w16, bias=self.proj.b)                # project_to_mel (model.py:249)
         pe = self.m.encoder.positional_encoding.pos_embedding[0]
-        x32, x16 = self._gemm_dual(x0, self.dense.w16, residual=pe, res_row_mod=S,
+        x32, x16 = self._gemm_dual(x0, self.dense, residual=pe, res_row_mod=S,
                                    drop=self.D("enc.pe"), drop_after_residual=True)   # dense + PE + dropout (model.py:130-132)
         if save is not None:
             save.append(dict(mel16=mel16, x0=x0, B=B, S=S))
@@ -336,16 +366,15 @@ class _Engine:
         res = dict(residual=x32)
         for li, L in enumerate(self.enc):
             p = L["p"]
-            qkv = K.gemm(x16, L["sa"].w16, bias=L["sa"].b)
+            qkv = self._lin(x16, L["sa"])
             attn, lse = K.attn_fwd(qkv[:, :d], qkv[:, d:2 * d], qkv[:, 2 * d:], B, H, S, S, self.scale, drop=self.D(p + ".attn"), head_dim=self.dh,
                                    save_bits=save is not None)
-            y1 = K.gemm(attn, L["sa_o"].w16, bias=L["sa_o"].b, out_dtype=F32, drop=self.D(p + ".drop1"), **res)
+            y1 = self._lin(attn, L["sa_o"], out_dtype=F32, drop=self.D(p + ".drop1"), **res)
             g1, b1 = self.P(p + ".norm1.weight"), self.P(p + ".norm1.bias")
             x1_32, x1_16, mean1, rstd1 = self._ln(y1, g1, b1, want32=not lean)
             res = dict(residual=y1, residual_ln=(mean1, rstd1, g1, b1)) if lean else dict(residual=x1_32)
-            u = torch.empty((M, L["l1"].w16.shape[0]), dtype=self.adt, device=src.device)
-            h = K.gemm(x1_16, L["l1"].w16, bias=L["l1"].b, act=1, act_grad_out=u, drop=self.D(p + ".ffn"))
-            y2 = K.gemm(h, L["l2"].w16, bias=L["l2"].b, out_dtype=F32, drop=self.D(p + ".drop2"), **res)
+            u, h = self._ffn1(x1_16, L["l1"], p)
+            y2 = self._lin(h, L["l2"], out_dtype=F32, drop=self.D(p + ".drop2"), **res)
             g2, b2 = self.P(p + ".norm2.weight"), self.P(p + ".norm2.bias")
             last = li + 1 == len(self.enc)                                 # the final LayerNorm reads this one's fp32 output
             x2_32, x2_16, mean2, rstd2 = self._ln(y2, g2, b2, want32=last or not lean)
@@ -373,32 +402,31 @@ class _Engine:
         # slices of one [B*S, layers*2d] buffer.  What this buys is in the backward: the memory's gradient becomes ONE product
         # with K = layers * 2d instead of a chain of GEMMs that each re-read and re-write the fp32 [B*S, d] accumulator.
         kv_all = None
-        if not self.fp32 and len(self.dec) > 1 and not os.environ.get("ADT_NO_KV_BATCH"):
+        if not self.fp32 and not self.int8 and len(self.dec) > 1 and not os.environ.get("ADT_NO_KV_BATCH"):
             wkv, bkv, _ = self._kv_operands()
             kv_all = K.gemm(mem16, wkv, bias=bkv)
+        mem = self._quant(mem16) if kv_all is None else mem16
         lean = self._lean_ln()
         res = dict(residual=x32)
         for li, L in enumerate(self.dec):
             p = L["p"]
-            qkv = K.gemm(x16, L["sa"].w16, bias=L["sa"].b)
+            qkv = self._lin(x16, L["sa"])
             sa, lse_s = K.attn_fwd(qkv[:, :d], qkv[:, d:2 * d], qkv[:, 2 * d:], B, H, T, T, self.scale, causal=True, key_len=key_len,
                                    drop=self.D(p + ".sattn"), head_dim=self.dh, save_bits=save is not None)
-            y1 = K.gemm(sa, L["sa_o"].w16, bias=L["sa_o"].b, out_dtype=F32, drop=self.D(p + ".drop1"), **res)
+            y1 = self._lin(sa, L["sa_o"], out_dtype=F32, drop=self.D(p + ".drop1"), **res)
             g1, b1 = self.P(p + ".norm1.weight"), self.P(p + ".norm1.bias")
             x1_32, x1_16, mean1, rstd1 = self._ln(y1, g1, b1, want32=not lean)
             res = dict(residual=y1, residual_ln=(mean1, rstd1, g1, b1)) if lean else dict(residual=x1_32)
-            ca_w, ca_b = L["ca"].w16, L["ca"].b
-            qc = K.gemm(x1_16, ca_w[:d], bias=ca_b[:d])
-            kvc = kv_all[:, 2 * d * li:2 * d * (li + 1)] if kv_all is not None else K.gemm(mem16, ca_w[d:], bias=ca_b[d:])
+            qc = self._lin(x1_16, L["ca"], None, d)
+            kvc = kv_all[:, 2 * d * li:2 * d * (li + 1)] if kv_all is not None else self._lin(mem, L["ca"], d, None)
             ca, lse_c = K.attn_fwd(qc, kvc[:, :d], kvc[:, d:], B, H, T, S, self.scale, drop=self.D(p + ".cattn"), head_dim=self.dh,
                                    save_bits=save is not None)
-            y2 = K.gemm(ca, L["ca_o"].w16, bias=L["ca_o"].b, out_dtype=F32, drop=self.D(p + ".drop2"), **res)
+            y2 = self._lin(ca, L["ca_o"], out_dtype=F32, drop=self.D(p + ".drop2"), **res)
             g2, b2 = self.P(p + ".norm2.weight"), self.P(p + ".norm2.bias")
             x2_32, x2_16, mean2, rstd2 = self._ln(y2, g2, b2, want32=not lean)
             res = dict(residual=y2, residual_ln=(mean2, rstd2, g2, b2)) if lean else dict(residual=x2_32)
-            u = torch.empty((Md, L["l1"].w16.shape[0]), dtype=self.adt, device=dev)
-            h = K.gemm(x2_16, L["l1"].w16, bias=L["l1"].b, act=1, act_grad_out=u, drop=self.D(p + ".ffn"))
-            y3 = K.gemm(h, L["l2"].w16, bias=L["l2"].b, out_dtype=F32, drop=self.D(p + ".drop3"), **res)
+            u, h = self._ffn1(x2_16, L["l1"], p)
+            y3 = self._lin(h, L["l2"], out_dtype=F32, drop=self.D(p + ".drop3"), **res)
             g3, b3 = self.P(p + ".norm3.weight"), self.P(p + ".norm3.bias")
             x3_32, x3_16, mean3, rstd3 = self._ln(y3, g3, b3, want32=not lean)
             res = dict(residual=y3, residual_ln=(mean3, rstd3, g3, b3)) if lean else dict(residual=x3_32)
@@ -425,6 +453,8 @@ class _Engine:
     # ---- loss + gradients ---------------------------------------------------------------
     def loss_and_grads(self, src, tgt, tgt_padding_mask, labels, want_grads=True, return_logits=False):
         """Full training step arithmetic.  Gradients land in ``self.G`` (views of ``self.gflat``)."""
+        if self.int8 and (want_grads or (self.m.training and self.m.config.dropout > 0)):
+            raise RuntimeError('precision "int8" is for inference: no backward pass and no dropout (model.eval() under torch.no_grad())')
         self.refresh_weights()
         self.drop_p = float(self.m.config.dropout) if self.m.training else 0.0
         if self.drop_p > 0.0:
@@ -587,7 +617,7 @@ class _Engine:
 
     @torch.no_grad()
     def greedy_decode_cached(self, mem16, B, S, max_length: int, start_token: int, end_token: int, sync_every: int = 16,
-                             use_graph: bool = True):
+                             use_graph: bool = True, kv_bits: int = 16):
         """KV-cached greedy decoding (hot-path row f1): the same arithmetic as running ``_decoder_fwd`` over the whole
         prefix at every step (model.py:300-322), but each step pushes ONE position through the decoder.
 
@@ -601,16 +631,28 @@ class _Engine:
         0.89 ms/step for the full-prefix recompute at 256 tokens; round 2, before the skinny-M GEMM and the single-query
         attention kernel: 0.68-0.83 ms/step replayed).  The host
         looks at the "all rows finished" flag every ``sync_every`` steps (the reference syncs every step).
+        ``kv_bits=4``: both caches -- the positions decoded so far and the memory's projections -- are held in 4 bits (``kernels.KV4Cache``, 72
+        bytes per row and head instead of 256) and read by ``attn_kv4``; bf16 activations only.
         Returns ``[B, n]`` tokens, n as the reference would stop."""
+        if kv_bits not in (4, 16) or (kv_bits == 4 and self.fp32):
+            raise ValueError('kv_bits is 16 (the activations\' own type) or 4, and 4 goes with precision "bf16" or "int8"')
         K.set_f32_products(self.products)
         d, H, dev = self.d, self.H, mem16.device
         Tmax = int(max_length)
+        kv4 = kv_bits == 4
         emb = self.P("decoder.tgt_tok_emb.embedding.weight")
         pe = self.m.decoder.positional_encoding.pos_embedding[0]
         if Tmax > pe.shape[0]:
             raise ValueError(f"max_length {Tmax} exceeds the positional table ({pe.shape[0]})")
-        caches = [torch.zeros((B, Tmax, 3 * d), dtype=self.adt, device=dev) for _ in self.dec]
-        kvcs = [K.gemm(mem16, L["ca"].w16[d:], bias=L["ca"].b[d:]) for L in self.dec]
+        mem = self._quant(mem16)
+        kvcs = [self._lin(mem, L["ca"], d, None) for L in self.dec]
+        if kv4:
+            caches = [K.KV4Cache(B, Tmax, H, self.dh, dev) for _ in self.dec]
+            for li, kvc in enumerate(kvcs):
+                kvcs[li] = K.KV4Cache(B, S, H, self.dh, dev)
+                K.kv4_append(kvcs[li], kvc[:, :d], kvc[:, d:])
+        else:
+            caches = [torch.zeros((B, Tmax, 3 * d), dtype=self.adt, device=dev) for _ in self.dec]
         gen = torch.full((B, Tmax), end_token, dtype=torch.long, device=dev)
         gen[:, 0] = start_token
         st = dict(tok=gen[:, :1].clone(), t=torch.zeros(1, dtype=torch.long, device=dev),
@@ -620,7 +662,7 @@ class _Engine:
 
         # LayerNorm -> projection pairs in one launch (adt_ln_gemm_bf16): every LayerNorm output of the step feeds exactly one GEMM as
         # its operand and one later GEMM as the residual, so the step's twelve LayerNorm launches fold into their consumers
-        fuse_ln = not self.fp32 and B <= 64 and d % 128 == 0 and d <= 1024 and not os.environ.get("ADT_NO_LN_GEMM")
+        fuse_ln = not self.fp32 and not self.int8 and B <= 64 and d % 128 == 0 and d <= 1024 and not os.environ.get("ADT_NO_LN_GEMM")
 
         def step():
             t = st["t"]
@@ -629,24 +671,31 @@ class _Engine:
             for li, (L, cache, kvc) in enumerate(zip(self.dec, caches, kvcs)):
                 p = L["p"]
                 if qkv is None:
-                    qkv = K.gemm(x16, L["sa"].w16, bias=L["sa"].b)                         # [B, 3d] of position t
-                cache.index_copy_(1, t, qkv.unsqueeze(1))
-                flat = cache.view(B * Tmax, 3 * d)
-                sa, _ = K.attn_fwd(qkv[:, :d], flat[:, d:2 * d], flat[:, 2 * d:], B, H, 1, Tmax, self.scale, key_len=st["klen"], head_dim=self.dh)
-                y1 = K.gemm(sa, L["sa_o"].w16, bias=L["sa_o"].b, residual=x32, out_dtype=F32)
+                    qkv = self._lin(x16, L["sa"])                                          # [B, 3d] of position t
+                if kv4:                                                                    # klen counts this position
+                    K.kv4_append(cache, qkv[:, d:2 * d], qkv[:, 2 * d:], st["klen"])
+                    sa = K.attn_kv4(qkv[:, :d], cache, st["klen"], heads=H, scale=self.scale)
+                else:
+                    cache.index_copy_(1, t, qkv.unsqueeze(1))
+                    flat = cache.view(B * Tmax, 3 * d)
+                    sa, _ = K.attn_fwd(qkv[:, :d], flat[:, d:2 * d], flat[:, 2 * d:], B, H, 1, Tmax, self.scale, key_len=st["klen"], head_dim=self.dh)
+                y1 = self._lin(sa, L["sa_o"], residual=x32, out_dtype=F32)
                 if fuse_ln:
                     qc, x1_32 = K.ln_gemm(y1, self.P(p + ".norm1.weight"), self.P(p + ".norm1.bias"), L["ca"].w16[:d], bias=L["ca"].b[:d])
                 else:
                     x1_32, x1_16, _, _ = self._ln(y1, self.P(p + ".norm1.weight"), self.P(p + ".norm1.bias"))
-                    qc = K.gemm(x1_16, L["ca"].w16[:d], bias=L["ca"].b[:d])
-                ca, _ = K.attn_fwd(qc, kvc[:, :d], kvc[:, d:], B, H, 1, S, self.scale, head_dim=self.dh)
-                y2 = K.gemm(ca, L["ca_o"].w16, bias=L["ca_o"].b, residual=x1_32, out_dtype=F32)
+                    qc = self._lin(x1_16, L["ca"], None, d)
+                if kv4:
+                    ca = K.attn_kv4(qc, kvc, heads=H, scale=self.scale)
+                else:
+                    ca, _ = K.attn_fwd(qc, kvc[:, :d], kvc[:, d:], B, H, 1, S, self.scale, head_dim=self.dh)
+                y2 = self._lin(ca, L["ca_o"], residual=x1_32, out_dtype=F32)
                 if fuse_ln:
                     h, x2_32 = K.ln_gemm(y2, self.P(p + ".norm2.weight"), self.P(p + ".norm2.bias"), L["l1"].w16, bias=L["l1"].b, act=1)
                 else:
                     x2_32, x2_16, _, _ = self._ln(y2, self.P(p + ".norm2.weight"), self.P(p + ".norm2.bias"))
-                    h = K.gemm(x2_16, L["l1"].w16, bias=L["l1"].b, act=1)
-                y3 = K.gemm(h, L["l2"].w16, bias=L["l2"].b, residual=x2_32, out_dtype=F32)
+                    h = self._lin(x2_16, L["l1"], act=1)
+                y3 = self._lin(h, L["l2"], residual=x2_32, out_dtype=F32)
                 n3w, n3b = self.P(p + ".norm3.weight"), self.P(p + ".norm3.bias")
                 if not fuse_ln:
                     x32, x16, _, _ = self._ln(y3, n3w, n3b)
@@ -759,7 +808,7 @@ class ADTModel(PreTrainedModel):
         return self
 
     def set_precision(self, precision: str) -> "ADTModel":
-        """``"bf16"`` (throughput default), ``"fp32"`` or ``"bf16x3"`` (the parity arms, see ``_Engine``)."""
+        """``"bf16"`` (throughput default), ``"fp32"`` or ``"bf16x3"`` (the parity arms), or ``"int8"`` (inference; see ``_Engine``)."""
         if precision not in PRECISIONS:
             raise ValueError(f"precision must be one of {PRECISIONS}, not {precision!r}")
         self._precision, self._engine_obj = precision, None
@@ -781,18 +830,20 @@ class ADTModel(PreTrainedModel):
 
     @torch.no_grad()
     def sample(self, src, src_mask=None, tgt_mask=None, max_length: int = 1000, start_token: int = 2, end_token: int = 3,
-               use_cache: bool = True):
+               use_cache: bool = True, kv_bits: int = 16):
         """Greedy decoding (model.py:260-324): encoder once, argmax of the last position, finished rows pinned to
         ``end_token``, stop when every row is finished.  ``use_cache=True`` (default) decodes one position per step
         against per-layer K/V caches; ``use_cache=False`` runs the full decoder over the prefix at every step exactly
-        like the reference (kept as the parity arm)."""
+        like the reference (kept as the parity arm).  ``kv_bits=4`` holds those caches in 4 bits (precision ``"bf16"`` or ``"int8"``)."""
         if not self.config.plain:
             raise NotImplementedError("Non-plain mode is not implemented")
+        if kv_bits != 16 and not use_cache:
+            raise ValueError("kv_bits is a property of the cached decode (use_cache=True)")
         self.eval()
         eng = self.engine
         mem16, B, S = eng.encode(src)
         if use_cache:
-            return eng.greedy_decode_cached(mem16, B, S, max_length, start_token, end_token)
+            return eng.greedy_decode_cached(mem16, B, S, max_length, start_token, end_token, kv_bits=kv_bits)
         gen = torch.full((B, 1), start_token, dtype=torch.long, device=src.device)
         finished = torch.zeros(B, dtype=torch.bool, device=src.device)
         for _ in range(max_length - 1):

@@ -1,4 +1,4 @@
-"""Drop-in for the reference's ``inference.py``: ``python inference.py <in.wav> <config.yaml> [-o dir] [-s]``.
+"""Drop-in for the reference's ``inference.py``: ``python inference.py <in.wav> <config.yaml> [-o dir] [-s] [--precision int8] [--kv-bits 4]``.
 
 load -> mono -> fixed chunks of ``input_sec`` (last one zero padded, inference.py:35-48) -> greedy ``sample`` ->
 ``decode`` -> notes shifted by the chunk start -> unique rows -> Standard MIDI File (+ optional re-synthesis).
@@ -23,17 +23,19 @@ def _chunk_audio(wav: torch.Tensor, chunk_samples: int):
     return out.view(n, chunk_samples)
 
 
-def transcribe(model, cfg: dict, wav: torch.Tensor, batch_size: int = 8, token_sink=None):
-    """``token_sink``: a list that receives the generated token ids of every chunk (one list of ints per chunk, in order)."""
+def transcribe(model, cfg: dict, wav: torch.Tensor, batch_size: int = 8, token_sink=None, kv_bits: int = 16):
+    """``token_sink``: a list that receives the generated token ids of every chunk (one list of ints per chunk, in order).
+    ``kv_bits=4``: the decode's K/V caches in 4 bits (``ADTModel.sample``)."""
     shared, inf = cfg["shared"], cfg["inference"]
     tok_cfg = cfg.get("tokenizer") or dict(ADTOF_mapping=False, BOS_token=2, EOS_token=3, pad_token=1, silence_token=0, add_velocity=True)
     tokenizer = MidiTokenizer(MidiTokenizerConfig(**tok_cfg))
     chunk = int(round(shared["input_sec"] * shared["sample_rate"]))
     chunks = _chunk_audio(wav, chunk)
     notes = []
+    few_bits = {} if kv_bits == 16 else dict(kv_bits=kv_bits)
     for i in range(0, chunks.shape[0], batch_size):
         ids = model.sample(src=chunks[i:i + batch_size], src_mask=None, tgt_mask=None, max_length=inf["max_length"],
-                           start_token=tok_cfg["BOS_token"], end_token=tok_cfg["EOS_token"]).cpu()
+                           start_token=tok_cfg["BOS_token"], end_token=tok_cfg["EOS_token"], **few_bits).cpu()
         for j, row in enumerate(ids):
             if token_sink is not None:
                 token_sink.append(row.tolist())
@@ -56,19 +58,24 @@ def _parser() -> argparse.ArgumentParser:
     ap.add_argument("-s", "--synthetise_transcription", "--synthesize", dest="synthesize", action="store_true",
                     help="Resynthesize the drum transcription with the one-shot mixer")
     ap.add_argument("--save-tokens", action="store_true", help="also write <stem>.tokens.json: the generated token ids per chunk")
+    ap.add_argument("--precision", default=None, choices=["bf16", "fp32", "bf16x3", "int8"], help="arithmetic of the network (default: ADT_PRECISION or bf16); "
+                    "int8: 8-bit-integer linear layers")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="4: K/V caches of the decode in 4 bits (precision bf16 or int8)")
     return ap
 
 
 def main():
     a = _parser().parse_args()
     model, cfg = build_model(a.config_path, device="cuda")
+    if a.precision:
+        model.set_precision(a.precision)
     audio, sr = read_wav(a.input_path)
     wav = torch.from_numpy(audio.mean(axis=0)).cuda()
     if sr != cfg["shared"]["sample_rate"]:                 # reference inference.py:88-90
         from adt_str_amd.resample import Resample
         wav = Resample(sr, cfg["shared"]["sample_rate"])(wav)
     tokens = [] if a.save_tokens else None
-    notes = transcribe(model, cfg, wav, cfg["inference"]["batch_size"], tokens)
+    notes = transcribe(model, cfg, wav, cfg["inference"]["batch_size"], tokens, a.kv_bits)
     os.makedirs(a.output_dir, exist_ok=True)
     stem = os.path.splitext(os.path.basename(a.input_path))[0]
     if tokens is not None:
