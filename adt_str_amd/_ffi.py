@@ -116,6 +116,8 @@ SIGNATURES = {
     "adt_embed_bwd_operands_f32": [ptr, ptr, f32, ptr, i64, ptr, i64, i64, i64, ptr, ptr],
     "adt_quant_rows_i8": [ptr, i32, i64, i64, i64, ptr, i64, ptr, ptr],
     "adt_gemm_i8": [i64, i64, i64, ptr, i64, ptr, ptr, i64, ptr, ptr, i64, ptr, ptr],
+    "adt_linear_i8_workspace_bytes": [i64, i64],
+    "adt_linear_i8": [i64, i64, i64, ptr, i32, i64, ptr, i64, ptr, ptr, i64, ptr, ptr, C.c_size_t, ptr],
     "adt_kv4_bytes": [i64, i32, i32, i64],
     "adt_kv4_append": [ptr, i64, i32, i32, i64, ptr, i64, ptr, i64, i64, ptr, ptr, ptr],
     "adt_kv4_read": [ptr, i64, i32, i32, i64, ptr, i64, ptr, i64, i32, i64, ptr, ptr, ptr],
@@ -153,7 +155,7 @@ _RESTYPES.update({n: C.c_size_t for n in ("adt_mix_workspace_bytes", "adt_gemm_w
                                           "adt_cross_entropy_workspace_bytes", "adt_grad_norm_workspace_bytes",
                                           "adt_htsat_fusion_embed_workspace_bytes",
                                           "adt_attn_bwd_f32_workspace_bytes", "adt_colsum_f32_workspace_bytes", "adt_gemm_f32_workspace_bytes",
-                                          "adt_gemm_bf16x3_workspace_bytes", "adt_kv4_bytes", "adt_attn_kv4_workspace_bytes")})
+                                          "adt_gemm_bf16x3_workspace_bytes", "adt_linear_i8_workspace_bytes", "adt_kv4_bytes", "adt_attn_kv4_workspace_bytes")})
 
 
 class AdtError(RuntimeError):

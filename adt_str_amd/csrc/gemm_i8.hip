@@ -7,6 +7,9 @@
 // The int8 matrix instruction (v_mfma_i32_16x16x64_i8) does twice the products of the bf16 one per cycle on the same operand bytes.
 #include <hip/hip_runtime.h>
 
+#include <cstdio>
+#include <cstdlib>
+
 #include "adt_common.h"
 
 namespace adt {
@@ -83,33 +86,60 @@ __device__ __forceinline__ void load8(const QuantArgs& a, long row, int k, bool 
     }
   }
 }
-__device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
+template <int kLanes>
+__device__ __forceinline__ unsigned lanes_max_u32(unsigned v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { const unsigned t = __shfl_xor(v, o); v = t > v ? t : v; }
+  for (int o = kLanes / 2; o > 0; o >>= 1) { const unsigned t = __shfl_xor(v, o); v = t > v ? t : v; }
   return v;
 }
-template <bool kF32>
-__global__ __launch_bounds__(256) void quant_rows_i8_kernel(QuantArgs a, bool vec) {
-  const int lane = threadIdx.x & 63;
-  const long row = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= a.M) return;
-  unsigned mx = 0;
-  for (int k = 8 * lane; k < a.Kp; k += 512) {
-    float v[8];
-    load8<kF32>(a, row, k, vec, v);
+__device__ __forceinline__ unsigned widest8(const float (&v)[8], unsigned mx) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { const unsigned t = __float_as_uint(v[j]) & 0x7fffffffu; mx = t > mx ? t : mx; }
+  for (int j = 0; j < 8; ++j) { const unsigned t = __float_as_uint(v[j]) & 0x7fffffffu; mx = t > mx ? t : mx; }
+  return mx;
+}
+template <bool kF32>
+__device__ __forceinline__ uint2 quant8(const float (&v)[8], const RowScale& s) {
+  unsigned q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = quant_code<kF32>(v[j], s);
+  return s.bad ? make_uint2(0u, 0u) : make_uint2(pack_bytes(q[0], q[1], q[2], q[3]), pack_bytes(q[4], q[5], q[6], q[7]));
+}
+// kLanes lanes per row, kP pieces of eight elements per lane held in registers from the maximum to the codes: one read of x.  kP = 0: any K,
+// the row is read twice.
+template <bool kF32, int kLanes, int kP>
+__global__ __launch_bounds__(256) void quant_rows_i8_kernel(QuantArgs a, bool vec) {
+  const int sub = threadIdx.x % kLanes;
+  const long row = static_cast<long>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  const bool live = row < a.M;
+  const long r = live ? row : a.M - 1;           // (lanes of rows past the last one take part in the exchanges)
+  float v[kP > 0 ? kP : 1][8];
+  unsigned mx = 0;
+  if constexpr (kP > 0) {
+#pragma unroll
+    for (int p = 0; p < kP; ++p) load8<kF32>(a, r, 8 * (sub + kLanes * p), vec, v[p]);
+#pragma unroll
+    for (int p = 0; p < kP; ++p) mx = widest8(v[p], mx);
+  } else {
+    for (int k = 8 * sub; k < a.Kp; k += 8 * kLanes) {
+      load8<kF32>(a, r, k, vec, v[0]);
+      mx = widest8(v[0], mx);
+    }
   }
   float sc;
-  const RowScale s = row_scale(wave_max_u32(mx), &sc);
-  if (lane == 0) a.scale[row] = sc;
-  for (int k = 8 * lane; k < a.Kp; k += 512) {
-    float v[8];
-    load8<kF32>(a, row, k, vec, v);
-    unsigned q[8];
+  const RowScale s = row_scale(lanes_max_u32<kLanes>(mx), &sc);
+  if (!live) return;
+  if (sub == 0) a.scale[row] = sc;
+  if constexpr (kP > 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = s.bad ? 0u : quant_code<kF32>(v[j], s);
-    *reinterpret_cast<uint2*>(a.q + row * a.ldq + k) = make_uint2(pack_bytes(q[0], q[1], q[2], q[3]), pack_bytes(q[4], q[5], q[6], q[7]));
+    for (int p = 0; p < kP; ++p) {
+      const int k = 8 * (sub + kLanes * p);
+      if (k < a.Kp) *reinterpret_cast<uint2*>(a.q + row * a.ldq + k) = quant8<kF32>(v[p], s);
+    }
+  } else {
+    for (int k = 8 * sub; k < a.Kp; k += 8 * kLanes) {
+      load8<kF32>(a, r, k, vec, v[0]);
+      *reinterpret_cast<uint2*>(a.q + row * a.ldq + k) = quant8<kF32>(v[0], s);
+    }
   }
 }
 
@@ -128,19 +158,30 @@ struct GemmI8Args {
 };
 __device__ __forceinline__ int w_row_bf16(int j, int i) { return 32 * (j >> 1) + 8 * (i >> 2) + 4 * (j & 1) + (i & 3); }
 
-template <bool kOut32, int kN>
-__device__ __forceinline__ void i8_store(const GemmI8Args& g, long m, int n, const int (&acc)[kN], float as, const float (&bs)[kN], const float (&bias)[kN]) {
+// What a call's epilogue is made of, as far as it is known when the kernel is compiled: everything at run time costs the 256 x 256 kernel 80 KB of
+// code, more than an instruction cache holds.
+__device__ __forceinline__ const float* i8_residual(const GemmI8Args& g, long m, int n) {
+  return g.residual + (g.res_row_mod ? static_cast<unsigned>(m) % static_cast<unsigned>(g.res_row_mod) : m) * g.ld_res + n;
+}
+constexpr int kI8Plain = 0, kI8Gelu = 1, kI8Residual = 2, kI8Any = 3;      // rows as GemmI8Args::vec, and no residual / copy except kI8Residual; kI8Any: whatever the call says
+template <bool kOut32, int kN, int kForm>
+__device__ __forceinline__ void i8_store(const GemmI8Args& g, long m, int n, const int (&acc)[kN], float as, const float (&bs)[kN], const float (&bias)[kN],
+                                         const float* ahead = nullptr) {      // ahead: the residual's kN values, where they were requested in front of the call
   float z[kN];
   const float* res = nullptr;
-  if (g.residual) res = g.residual + (g.res_row_mod ? m % g.res_row_mod : m) * g.ld_res + n;
-  const bool whole = g.vec && n + kN <= g.N;
+  if (kForm == kI8Any && g.residual) res = i8_residual(g, m, n);
+  const bool whole = kForm != kI8Any || (g.vec && n + kN <= g.N);      // (vec: N is a multiple of 8)
 #pragma unroll
   for (int e = 0; e < kN; ++e) {
     z[e] = static_cast<float>(acc[e]) * as * bs[e] + bias[e];
-    if (g.act == 1) z[e] = gelu_erf(z[e]);
-    else if (g.act == 2) z[e] = fmaxf(z[e], 0.f);
+    if (kForm == kI8Gelu || (kForm == kI8Any && g.act == 1)) z[e] = gelu_erf(z[e]);
+    else if (kForm == kI8Any && g.act == 2) z[e] = fmaxf(z[e], 0.f);
   }
   if (whole) {
+    if (kForm == kI8Residual) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) z[e] += ahead[e];
+    }
     if (res) {
 #pragma unroll
       for (int e = 0; e < kN; e += 4) {
@@ -158,7 +199,7 @@ __device__ __forceinline__ void i8_store(const GemmI8Args& g, long m, int n, con
     for (int e = 0; e < kN / 2; ++e) p[e] = i8_pack_bf2(z[2 * e], z[2 * e + 1]);
     unsigned short* h = kOut32 ? g.aux : static_cast<unsigned short*>(g.C);
     const long ldh = kOut32 ? g.ld_aux : g.ldc;
-    if (!kOut32 || h) {
+    if (!kOut32 || (kForm >= kI8Residual && h)) {
       if constexpr (kN == 8) *reinterpret_cast<u32x4*>(h + m * ldh + n) = u32x4{p[0], p[1], p[2], p[3]};
       else *reinterpret_cast<uint2*>(h + m * ldh + n) = make_uint2(p[0], p[1]);
     }
@@ -174,6 +215,35 @@ __device__ __forceinline__ void i8_store(const GemmI8Args& g, long m, int n, con
   }
 }
 
+// The results of kT token blocks (rows m0 + 16 t + li) over the lane's kN channels from n on; acc_of(t, e) names an accumulator, as_of(t) a
+// token's scale.  All residual rows are requested before the first of them is needed.
+template <bool kOut32, int kForm, int kT, typename AccOf, typename AsOf>
+__device__ __forceinline__ void i8_store_column(const GemmI8Args& g, long m0, int n, const float (&bs)[kOut32 ? 4 : 8], const float (&bias)[kOut32 ? 4 : 8],
+                                                AccOf acc_of, AsOf as_of) {
+  constexpr int kN = kOut32 ? 4 : 8;
+  float ahead[kForm == kI8Residual ? kT : 1][kN];
+  if constexpr (kForm == kI8Residual) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const long m = min(m0 + 16 * t, static_cast<long>(g.M) - 1);
+#pragma unroll
+      for (int e = 0; e < kN; e += 4) {
+        const f32x4 r = g.residual ? *reinterpret_cast<const f32x4*>(i8_residual(g, m, n) + e) : f32x4{0.f, 0.f, 0.f, 0.f};
+        ahead[t][e] = r[0]; ahead[t][e + 1] = r[1]; ahead[t][e + 2] = r[2]; ahead[t][e + 3] = r[3];
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+    const long m = m0 + 16 * t;
+    if (m >= g.M) continue;
+    int z[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) z[e] = acc_of(t, e);
+    i8_store<kOut32, kN, kForm>(g, m, n, z, as_of(t), bs, bias, ahead[kForm == kI8Residual ? t : 0]);
+  }
+}
+
 // ---- 128 x 128 tile, four waves (2 x 2, 64 x 64 each), K in steps of 128 bytes, two LDS stages filled by LDS-DMA
 constexpr int kI8Tile = 128 * 128;               // one operand's stage: 128 rows x 128 bytes
 constexpr int kI8Lds = 4 * kI8Tile;
@@ -182,7 +252,7 @@ __device__ __attribute__((aligned(16))) unsigned g_i8_zero[4];
 __device__ __forceinline__ int i8_swz_natural(int row) { return (row >> 1) & 7; }
 __device__ __forceinline__ int i8_swz_bf16(int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); }
 
-template <bool kOut32>
+template <bool kOut32, int kForm>
 __global__ __launch_bounds__(256) void gemm_i8_kernel(GemmI8Args g, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [2 stages][token tile | weight tile]
   const int tid = threadIdx.x, lane = tid & 63;
@@ -253,6 +323,9 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(GemmI8Args g, int tiles_m,
     __syncthreads();
   }
   constexpr int kN = kOut32 ? 4 : 8;
+  float as[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) as[j] = g.a_scale[min(m0 + wm * 64 + 16 * j + li, g.M - 1)];
 #pragma unroll
   for (int b = 0; b < 16 / kN; ++b) {            // the lane's groups of kN channels
     const int n = n0 + wn * 64 + (kOut32 ? 16 * b + 4 * lg : 32 * b + 8 * lg);
@@ -264,21 +337,377 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(GemmI8Args g, int tiles_m,
       bs[e] = g.b_scale[c];
       bias[e] = g.bias ? g.bias[c] : 0.f;
     }
+    i8_store_column<kOut32, kForm, 4>(g, m0 + wm * 64 + li, n, bs, bias,
+                                      [&](int j, int e) { return kOut32 ? acc[b][j][e & 3] : acc[2 * b + (e >> 2)][j][e & 3]; }, [&](int j) { return as[j]; });
+  }
+}
+
+// ---- few tokens: 16 kMT tokens x 16 channels per workgroup, K dealt in steps of 64 bytes over its eight waves, which join through LDS
+//
+// What bounds such a call is the time of a memory round trip, not its bytes, so a wave asks for the operands of several steps at once and there
+// is one launch where the rows still have to be quantised and are few (kX: x is bf16 or fp32): every workgroup then quantises the
+// rows for itself, 7 instructions a code, from the registers that hold its share of them (K up to 2048).
+constexpr int kI8SkinnyDepth = 4, kI8SkinnyWaves = 8;
+struct LinearX { const void* x; long ldx; int K; bool vec; };      // K columns of x; GemmI8Args::K is K rounded up to 16
+enum { kXInt8 = 0, kXBf16 = 1, kXF32 = 2 };
+template <bool kOut32, int kMT, int kX>
+__global__ __launch_bounds__(64 * kI8SkinnyWaves) void gemm_i8_skinny_kernel(GemmI8Args g, LinearX lx) {
+  static_assert(kX == kXInt8 || kMT == 1, "rows are quantised here for one block of tokens");
+  constexpr int kW = kI8SkinnyWaves;
+  __shared__ int part[kW][16 * kMT][20];
+  __shared__ unsigned smax[kW][16];
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * kMT;
+  const int steps = (g.K + 63) >> 6;
+  // what the end needs is asked for at the start: four channels of one token per thread
+  const int er = tid >> 2, en = n0 + 4 * (tid & 3);
+  const long em = m0 + er;
+  const bool mine = tid < 64 * kMT && em < g.M && en < g.N;
+  float ebs[4], ebias[4], eas = 0.f;
+  if (mine) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const long m = m0 + wm * 64 + 16 * j + li;
-      if (m >= g.M) continue;
-      int v[kN];
-#pragma unroll
-      for (int e = 0; e < kN; ++e) v[e] = kOut32 ? acc[b][j][e & 3] : acc[2 * b + (e >> 2)][j][e & 3];
-      i8_store<kOut32, kN>(g, m, n, v, g.a_scale[m], bs, bias);
+      const int c = min(en + j, g.N - 1);
+      ebs[j] = g.b_scale[c];
+      ebias[j] = g.bias ? g.bias[c] : 0.f;
     }
+    if (kX == kXInt8) eas = g.a_scale[em];
   }
+  const signed char* pb = g.B + static_cast<long>(min(n0 + li, g.N - 1)) * g.ldb + 16 * lg;
+  const i32x4 zero = {0, 0, 0, 0};
+  i32x4 acc[kMT];
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) acc[t] = zero;
+  float a_own = 0.f;                             // kX: the scale of this lane's token
+  if constexpr (kX == kXInt8) {
+    const signed char* pa[kMT];
+#pragma unroll
+    for (int t = 0; t < kMT; ++t) pa[t] = g.A + static_cast<long>(min(m0 + 16 * t + li, g.M - 1)) * g.lda + 16 * lg;
+    for (int s0 = wave; s0 < steps; s0 += kW * kI8SkinnyDepth) {
+      i32x4 fb[kI8SkinnyDepth], fa[kMT][kI8SkinnyDepth];
+#pragma unroll
+      for (int i = 0; i < kI8SkinnyDepth; ++i) {
+        const int k = 64 * (s0 + kW * i);
+        const bool in = k + 16 * lg < g.K;         // the last step's pieces past K, and steps past the last one
+        fb[i] = in ? *reinterpret_cast<const i32x4*>(pb + k) : zero;
+#pragma unroll
+        for (int t = 0; t < kMT; ++t) fa[t][i] = in ? *reinterpret_cast<const i32x4*>(pa[t] + k) : zero;
+      }
+#pragma unroll
+      for (int i = 0; i < kI8SkinnyDepth; ++i)
+#pragma unroll
+        for (int t = 0; t < kMT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[i], fa[t][i], acc[t], 0, 0, 0);
+    }
+  } else {
+    const QuantArgs qa{lx.x, lx.ldx, nullptr, 0, nullptr, g.M, lx.K, g.K};
+    const long row = min(m0 + li, g.M - 1);
+    float held[kI8SkinnyDepth][16];
+    i32x4 fb[kI8SkinnyDepth];
+    auto load16 = [&](int s, float (&v)[16]) {
+      float lo[8], hi[8];
+      load8<kX == kXF32>(qa, row, 64 * s + 16 * lg, lx.vec, lo);
+      load8<kX == kXF32>(qa, row, 64 * s + 16 * lg + 8, lx.vec, hi);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { v[j] = lo[j]; v[8 + j] = hi[j]; }
+    };
+    unsigned mx = 0;
+    auto widen = [&](const float (&v)[16]) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) { const unsigned t = __float_as_uint(v[j]) & 0x7fffffffu; mx = t > mx ? t : mx; }
+    };
+#pragma unroll
+    for (int i = 0; i < kI8SkinnyDepth; ++i) {     // (past K: zeros)
+      const int s = wave + kW * i, k = 64 * s;
+      fb[i] = k + 16 * lg < g.K ? *reinterpret_cast<const i32x4*>(pb + k) : zero;
+      if (s < steps) load16(s, held[i]);         // (wave-uniform)
+    }
+#pragma unroll
+    for (int i = 0; i < kI8SkinnyDepth; ++i)
+      if (wave + kW * i < steps) widen(held[i]);
+    { const unsigned a = __shfl_xor(mx, 16); mx = a > mx ? a : mx; }
+    { const unsigned a = __shfl_xor(mx, 32); mx = a > mx ? a : mx; }
+    if (lg == 0) smax[wave][li] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kW; ++w) mx = smax[w][li] > mx ? smax[w][li] : mx;
+    const RowScale rs = row_scale(mx, &a_own);
+    auto codes = [&](const float (&v)[16]) {
+      i32x4 f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned w = pack_bytes(quant_code<kX == kXF32>(v[4 * q], rs), quant_code<kX == kXF32>(v[4 * q + 1], rs), quant_code<kX == kXF32>(v[4 * q + 2], rs),
+                                      quant_code<kX == kXF32>(v[4 * q + 3], rs));
+        f[q] = rs.bad ? 0 : static_cast<int>(w);
+      }
+      return f;
+    };
+#pragma unroll
+    for (int i = 0; i < kI8SkinnyDepth; ++i)
+      if (wave + kW * i < steps) acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[i], codes(held[i]), acc[0], 0, 0, 0);
+  }
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) *reinterpret_cast<i32x4*>(&part[wave][16 * t + li][4 * lg]) = acc[t];
+  __shared__ float srow[16];
+  if (kX != kXInt8 && wave == 0 && lg == 0) srow[li] = a_own;
+  __syncthreads();
+  if (!mine) return;
+  int z[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = 4 * (tid & 3) + j;
+    z[j] = 0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) z[j] += part[w][er][c];
+  }
+  i8_store<kOut32, 4, kI8Any>(g, em, en, z, kX == kXInt8 ? eas : srow[er & 15], ebs, ebias);
+}
+
+// ---- 256 x 256 tile, eight waves (2 x 4, 128 tokens x 64 channels each), K in steps of 128 bytes, one persistent workgroup per CU
+//
+// LDS: two buffers of four half-tiles of 128 rows x 128 bytes,
+//     A_h: token rows wr 128 + 64 h + 0..63 of the tile for the wave rows wr = 0, 1;  B_h: weight rows wc 64 + 32 h + 0..31 for the wave columns wc = 0..3
+// so that a half-tile is consumed in one phase by all waves.  A K-step is four phases of 16 products per wave:
+//     phase 1: read B_0, A_0   products (A_0, B_0)   fetch A_1 of step t + 1
+//     phase 2: read B_1        products (A_0, B_1)   fetch B_0 of step t + 2
+//     phase 3: read A_1        products (A_1, B_1)   fetch A_0 of step t + 2
+//     phase 4:                 products (A_1, B_0)   fetch B_1 of step t + 2
+// In front of its first barrier a phase waits for what the next one reads and for no more: five half-tiles (80 KB) stay in flight, which
+// is what the loop's rate hangs on (the latency of a loaded L2 is more than a microsecond).
+// The wave rows run one barrier apart, so that one row's LDS reads and fetches lie under the other row's products on the same SIMDs.
+// A fetched half is read at least a phase after the wait that retires it; it is fetched into again two phases after its last read, or one
+// phase after where those reads were retired in front of that phase's barrier (B_0).  Barriers are raw, a __syncthreads would drain the
+// fetches.  Steps past the end fetch the last one again into halves that nobody reads, so that the counts stay exact.
+// Tiles are dealt statically: the workgroups of an XCD (block index modulo 8) walk one contiguous eighth of the tiles, in groups of a few tile
+// columns; no counters, so a captured launch is like any other.  The next tile's first fetches, its scales among them, are issued before this
+// tile's results are scaled and stored, which needs no LDS tile of its own.
+constexpr int kI8Half = 128 * 128;
+constexpr int kI8Buf = 4 * kI8Half;              // A_0 | A_1 | B_0 | B_1
+constexpr int kI8Scales = 3 * 256 * 4;           // a_scale | b_scale | bias of a tile
+constexpr int kI8BigLds = 2 * kI8Buf + 2 * kI8Scales;
+__device__ __forceinline__ unsigned i8_lds_addr(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
+}
+// LDS-DMA as inline asm without results: through the builtin the compiler takes every later LDS read to depend on it and waits for all
+// fetches in front of it.  The waits are the explicit ones of the schedule.
+__device__ __forceinline__ void i8_dma16(const void* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void i8_dma4(const void* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(src), "s"(lds) : "memory");
+}
+
+template <bool kOut32, int kForm>
+__global__ __launch_bounds__(512) void gemm_i8_256_kernel(GemmI8Args g, int tiles_m, int tiles_n, int group_n) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave >> 2, wc = wave & 3;
+  const int k_steps = (g.K + 127) >> 7;
+  const int n_tiles = tiles_m * tiles_n, xg = blockIdx.x & 7;
+  const int q8 = n_tiles >> 3, r8 = n_tiles & 7;
+  const int slice0 = xg < r8 ? xg * (q8 + 1) : r8 * (q8 + 1) + (xg - r8) * q8, slice_n = q8 + (xg < r8 ? 1 : 0);
+  const int stride = (static_cast<int>(gridDim.x) + 7 - xg) >> 3;
+  int v = blockIdx.x >> 3;
+  if (v >= slice_n) return;
+
+  // fetch j of this wave fills LDS rows 8 (2 wave + j) + (lane >> 3) of a half-tile, position p of row r holding the piece p ^ f(r)
+  const signed char *pa[2][2], *pb[2][2];        // [half][j]
+  int kca[2], kcb[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 8 * (2 * wave + j) + (lane >> 3);
+    kca[j] = ((lane & 7) ^ i8_swz_natural(r)) * 16;
+    kcb[j] = ((lane & 7) ^ (kOut32 ? i8_swz_natural(r) : i8_swz_bf16(r))) * 16;
+  }
+  const unsigned lds0 = i8_lds_addr(smem);
+  auto set_tile = [&](int v_, int& m0, int& n0) {
+    const int logical = slice0 + v_;
+    const int per_group = tiles_m * group_n;
+    const int cg = logical / per_group, rem = logical - cg * per_group;
+    const int gw = min(group_n, tiles_n - cg * group_n);
+    m0 = (rem / gw) * 256;
+    n0 = (cg * group_n + rem % gw) * 256;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 8 * (2 * wave + j) + (lane >> 3);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int ar = min(m0 + (r >> 6) * 128 + h * 64 + (r & 63), g.M - 1);
+        pa[h][j] = g.A + static_cast<long>(ar) * g.lda + kca[j];
+        const int br = min(n0 + (r >> 5) * 64 + h * 32 + (r & 31), g.N - 1);
+        pb[h][j] = g.B + static_cast<long>(br) * g.ldb + kcb[j];
+      }
+    }
+  };
+  auto dma = [&](const signed char* const (&p)[2], const int (&kc)[2], int step, int buf, int half) {
+    const int s = step < k_steps ? step : k_steps - 1;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const void* src = p[j] + static_cast<long>(s) * 128;
+      if (kForm == kI8Any) src = s * 128 + kc[j] < g.K ? src : static_cast<const void*>(g_i8_zero);      // (the other forms: K a multiple of 128)
+      i8_dma16(src, lds0 + buf * kI8Buf + half * kI8Half + (2 * wave + j) * 1024);
+    }
+  };
+  auto prologue = [&](int m0, int n0, int sbuf) {      // the tile's scales; step 0 whole; B_0, A_0, B_1 of step 1
+    const unsigned sl = lds0 + 2 * kI8Buf + sbuf * kI8Scales + (wave & 3) * 256;
+    if (wave < 4) {
+      i8_dma4(g.a_scale + min(m0 + 64 * wave + lane, g.M - 1), sl);
+    } else {
+      const int n = min(n0 + 64 * (wave - 4) + lane, g.N - 1);
+      i8_dma4(g.b_scale + n, sl + 1024);
+      if (g.bias) i8_dma4(g.bias + n, sl + 2048);
+    }
+    dma(pb[0], kcb, 0, 0, 2); dma(pa[0], kca, 0, 0, 0); dma(pb[1], kcb, 0, 0, 3); dma(pa[1], kca, 0, 0, 1);
+    dma(pb[0], kcb, 1, 1, 2); dma(pa[0], kca, 1, 1, 0); dma(pb[1], kcb, 1, 1, 3);
+  };
+  // fragment reads (byte offsets in a half-tile): token rows wr 64 + 16 i + li; weight rows wc 32 + (bf16 outputs: 8 (li / 4) + 4 j + (li & 3), fp32: 16 j + li)
+  const int sw = (li >> 1) & 7;
+  const int c0 = (lg ^ sw) * 16, c1 = c0 ^ 64;
+  const int a_off = (wr * 64 + li) * 128;
+  const int b_off = 2 * kI8Half + (wc * 32 + (kOut32 ? li : 8 * (li >> 2) + (li & 3))) * 128;
+  constexpr int kBj = kOut32 ? 16 * 128 : 4 * 128;
+  i32x4 fa[4][2], fb0[2][2], fb1[2][2];
+#define ADT_I8_READ_A(H)                                                                                   \
+  _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                                          \
+    fa[i][0] = *reinterpret_cast<const i32x4*>(st + a_off + c0 + (H) * kI8Half + i * 2048);                 \
+    fa[i][1] = *reinterpret_cast<const i32x4*>(st + a_off + c1 + (H) * kI8Half + i * 2048);                 \
+  }
+#define ADT_I8_READ_B(F, H)                                                                                \
+  _Pragma("unroll") for (int j = 0; j < 2; ++j) {                                                          \
+    F[j][0] = *reinterpret_cast<const i32x4*>(st + b_off + c0 + (H) * kI8Half + j * kBj);                   \
+    F[j][1] = *reinterpret_cast<const i32x4*>(st + b_off + c1 + (H) * kI8Half + j * kBj);                   \
+  }
+// What the next phase reads has landed when the five half-tiles asked for after it, ten fetches of this wave, are all that is in flight -- or those
+// and the stores that stand between them in the order of issue (a tile's first phases after an interior tile).
+#define ADT_I8_LANDED(BEHIND_STORES)                                                                       \
+  do {                                                                                                     \
+    if (stored && (BEHIND_STORES)) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(10 + kStores) : "memory");     \
+    else asm volatile("s_waitcnt vmcnt(10)" ::: "memory");                                                 \
+  } while (0)
+#define ADT_I8_QUAD(I0, FB, J0)                                                                            \
+  do {                                                                                                     \
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                     \
+    __builtin_amdgcn_sched_barrier(0);                                                                     \
+    __builtin_amdgcn_s_setprio(1);                                                                         \
+    _Pragma("unroll") for (int ks = 0; ks < 2; ++ks)                                                       \
+      _Pragma("unroll") for (int i = 0; i < 4; ++i)                                                        \
+        _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                      \
+          acc[I0 + i][J0 + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(FB[j][ks], fa[i][ks], acc[I0 + i][J0 + j], 0, 0, 0); \
+    __builtin_amdgcn_s_setprio(0);                                                                         \
+    __builtin_amdgcn_sched_barrier(0);                                                                     \
+    asm volatile("s_barrier" ::: "memory");                                                                \
+  } while (0)
+
+  constexpr int kStores = kOut32 ? 32 : 16;      // 16-byte stores of a wave's 128 x 64 results
+  int m0, n0, sbuf = 0;
+  set_tile(v, m0, n0);
+  prologue(m0, n0, 0);
+  asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+  bool stored = false;                           // the tile before left its last stores in flight
+  asm volatile("s_barrier" ::: "memory");
+  while (true) {
+    i32x4 acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    if (wr == 1) asm volatile("s_barrier" ::: "memory");
+    for (int t = 0; t < k_steps; ++t) {
+      const int buf = t & 1;
+      const unsigned char* st = smem + buf * kI8Buf;
+      ADT_I8_READ_B(fb0, 0)
+      __builtin_amdgcn_sched_barrier(0);
+      ADT_I8_READ_A(0)
+      dma(pa[1], kca, t + 1, buf ^ 1, 1);
+      asm volatile("s_waitcnt lgkmcnt(8)" ::: "memory");           // the B_0 reads: B_0 is fetched into in phase 2
+      ADT_I8_LANDED(t <= 1);
+      asm volatile("s_barrier" ::: "memory");
+      ADT_I8_QUAD(0, fb0, 0);
+      ADT_I8_READ_B(fb1, 1)
+      dma(pb[0], kcb, t + 2, buf, 2);
+      ADT_I8_LANDED(t == 0);
+      asm volatile("s_barrier" ::: "memory");
+      ADT_I8_QUAD(0, fb1, 2);
+      ADT_I8_READ_A(1)
+      dma(pa[0], kca, t + 2, buf, 0);
+      asm volatile("s_barrier" ::: "memory");
+      ADT_I8_QUAD(4, fb1, 2);
+      dma(pb[1], kcb, t + 2, buf, 3);
+      ADT_I8_LANDED(t == 0);
+      asm volatile("s_barrier" ::: "memory");
+      ADT_I8_QUAD(4, fb0, 0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (wr == 0) asm volatile("s_barrier" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");        // every fetch has landed and every fragment is read: the buffers are free
+    const int em0 = m0, en0 = n0;
+    const float* const scales = reinterpret_cast<const float*>(smem + 2 * kI8Buf + sbuf * kI8Scales);
+    v += stride;
+    const bool more = v < slice_n;                 // block-uniform
+    if (more) {
+      sbuf ^= 1;
+      set_tile(v, m0, n0);
+      prologue(m0, n0, sbuf);
+    }
+    float as[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) as[i] = scales[wr * 128 + 16 * i + li];
+    constexpr int kN = kOut32 ? 4 : 8;
+#pragma unroll
+    for (int b = 0; b < 16 / kN; ++b) {
+      const int nl = wc * 64 + (kOut32 ? 16 * b + 4 * lg : 32 * b + 8 * lg), n = en0 + nl;
+      if (n >= g.N) continue;
+      float bs[kN], bias[kN];
+#pragma unroll
+      for (int e = 0; e < kN; ++e) { bs[e] = scales[256 + nl + e]; bias[e] = g.bias ? scales[512 + nl + e] : 0.f; }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        i8_store_column<kOut32, kForm, 4>(g, em0 + wr * 128 + 64 * h + li, n, bs, bias,
+                                          [&](int i, int e) { return kOut32 ? acc[4 * h + i][b][e & 3] : acc[4 * h + i][2 * b + (e >> 2)][e & 3]; },
+                                          [&](int i) { return as[4 * h + i]; });
+    }
+    if (!more) break;
+    // The next tile's first fetches are older than this tile's stores, and a wave of an interior tile has just issued kStores of those at least: they
+    // may stay in flight under the next tile's first steps.  A wave of an edge tile may have issued none.
+    stored = em0 + 256 <= g.M && en0 + 256 <= g.N;
+    if (stored) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(10 + kStores) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+  }
+#undef ADT_I8_READ_A
+#undef ADT_I8_READ_B
+#undef ADT_I8_QUAD
+#undef ADT_I8_LANDED
 }
 
 }  // namespace adt
 
 using namespace adt;
+
+namespace adt {
+// Lanes per row: the fewest that hold the row in at most three pieces each, so that no lane idles (768 columns: 32 lanes, three pieces)
+template <bool kF32, int kLanes, int kP>
+static void launch_quant_as(const QuantArgs& a, bool vec, hipStream_t st) {
+  constexpr int kRows = 256 / kLanes;
+  hipLaunchKernelGGL((quant_rows_i8_kernel<kF32, kLanes, kP>), dim3(static_cast<unsigned>((static_cast<long>(a.M) + kRows - 1) / kRows)), dim3(256), 0, st, a, vec);
+}
+template <bool kF32>
+static void launch_quant(const QuantArgs& a, bool vec, hipStream_t st) {
+  const int pieces = (a.Kp + 7) / 8;
+  if (pieces <= 16) launch_quant_as<kF32, 16, 1>(a, vec, st);
+  else if (pieces <= 32) launch_quant_as<kF32, 16, 2>(a, vec, st);
+  else if (pieces <= 48) launch_quant_as<kF32, 16, 3>(a, vec, st);
+  else if (pieces <= 64) launch_quant_as<kF32, 32, 2>(a, vec, st);
+  else if (pieces <= 96) launch_quant_as<kF32, 32, 3>(a, vec, st);
+  else if (pieces <= 128) launch_quant_as<kF32, 64, 2>(a, vec, st);
+  else if (pieces <= 192) launch_quant_as<kF32, 64, 3>(a, vec, st);
+  else if (pieces <= 256) launch_quant_as<kF32, 64, 4>(a, vec, st);
+  else if (pieces <= 384) launch_quant_as<kF32, 64, 6>(a, vec, st);
+  else if (pieces <= 512) launch_quant_as<kF32, 64, 8>(a, vec, st);
+  else launch_quant_as<kF32, 64, 0>(a, vec, st);
+}
+}  // namespace adt
 
 extern "C" int adt_quant_rows_i8(const void* x, int32_t x_fp32, int64_t ldx, int64_t M, int64_t K, void* q, int64_t ldq, float* scale, void* stream) {
   if (!x || !q || !scale) return set_error(ADT_EINVAL, "adt_quant_rows_i8: null pointer");
@@ -288,39 +717,122 @@ extern "C" int adt_quant_rows_i8(const void* x, int32_t x_fp32, int64_t ldx, int
   if (M == 0) return ADT_OK;
   QuantArgs a{x, static_cast<long>(ldx), static_cast<signed char*>(q), static_cast<long>(ldq), scale, static_cast<int>(M), static_cast<int>(K), static_cast<int>(Kp)};
   const bool vec = aligned16(x) && (ldx * (x_fp32 ? 4 : 2)) % 16 == 0;
-  const dim3 grid(static_cast<unsigned>((M + 3) / 4));
-  if (x_fp32) hipLaunchKernelGGL(quant_rows_i8_kernel<true>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, vec);
-  else hipLaunchKernelGGL(quant_rows_i8_kernel<false>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, vec);
+  if (x_fp32) launch_quant<true>(a, vec, static_cast<hipStream_t>(stream));
+  else launch_quant<false>(a, vec, static_cast<hipStream_t>(stream));
   ADT_HIP_TRY(hipGetLastError());
   return ADT_OK;
 }
 
-extern "C" int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const float* a_scale, const void* B, int64_t ldb,
-                           const float* b_scale, void* C, int64_t ldc, const adt_gemm_epilogue* ep, void* stream) {
-  if (!A || !B || !C || !a_scale || !b_scale || !ep) return set_error(ADT_EINVAL, "adt_gemm_i8: null pointer");
-  if (M < 0 || N < 0 || K <= 0 || M > (1LL << 30) || N > (1LL << 30) || K > (1LL << 17) || (K & 15))
-    return set_error(ADT_ESHAPE, "adt_gemm_i8: K must be a multiple of 16, at most 131072 (the int32 sums stay exact)");
-  if (lda < K || ldb < K || ldc < N || (lda & 15) || (ldb & 15) || !aligned16(A) || !aligned16(B))
-    return set_error(ADT_EINVAL, "adt_gemm_i8: operand rows are 16-byte aligned; lda, ldb >= K, ldc >= N");
-  if (ep->act < 0 || ep->act > 2 || ep->alpha != 1.0f) return set_error(ADT_EINVAL, "adt_gemm_i8: act is 0, 1 or 2 and alpha 1");
+namespace adt {
+static int gemm_i8_check(const char* who, int64_t M, int64_t N, int64_t K, const void* B, int64_t ldb, const float* b_scale, const void* C, int64_t ldc,
+                         const adt_gemm_epilogue* ep) {
+  static thread_local char msg[200];
+  auto fail = [&](int code, const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", who, what);
+    return set_error(code, msg);
+  };
+  if (!B || !C || !b_scale || !ep) return fail(ADT_EINVAL, "null pointer");
+  if (M < 0 || N < 0 || K <= 0 || M > (1LL << 30) || N > (1LL << 30) || K > (1LL << 17)) return fail(ADT_ESHAPE, "M and N fit 30 bits, 1 <= K <= 131072 (the int32 sums stay exact)");
+  if (ldb < (K + 15) / 16 * 16 || ldc < N || (ldb & 15) || !aligned16(B)) return fail(ADT_EINVAL, "weight rows are 16-byte aligned and hold K rounded up to 16; ldc >= N");
+  if (ep->act < 0 || ep->act > 2 || ep->alpha != 1.0f) return fail(ADT_EINVAL, "act is 0, 1 or 2 and alpha 1");
   if (ep->gelu_grad_of || ep->pre_act_out || ep->colsum_out || ep->res_ln_mean || ep->drop.p > 0.f || ep->act_grad_mode || ep->side_fp32)
-    return set_error(ADT_EINVAL, "adt_gemm_i8: an inference product (bias, activation, residual, bf16 copy); the training epilogues are not its own");
-  if (ep->aux_bf16_out && !ep->out_fp32) return set_error(ADT_EINVAL, "adt_gemm_i8: aux_bf16_out goes with an fp32 C");
-  if (ep->residual && (ep->res_row_mod < 0 || ep->ld_res < N)) return set_error(ADT_EINVAL, "adt_gemm_i8: residual rows hold N floats");
-  if (ep->aux_bf16_out && ep->ld_aux < N) return set_error(ADT_EINVAL, "adt_gemm_i8: aux rows hold N elements");
-  if (M == 0 || N == 0) return ADT_OK;
+    return fail(ADT_EINVAL, "an inference product (bias, activation, residual, bf16 copy); the training epilogues are not its own");
+  if (ep->aux_bf16_out && !ep->out_fp32) return fail(ADT_EINVAL, "aux_bf16_out goes with an fp32 C");
+  if (ep->residual && (ep->res_row_mod < 0 || ep->ld_res < N)) return fail(ADT_EINVAL, "residual rows hold N floats");
+  if (ep->aux_bf16_out && ep->ld_aux < N) return fail(ADT_EINVAL, "aux rows hold N elements");
+  return ADT_OK;
+}
+static GemmI8Args gemm_i8_args(int64_t M, int64_t N, int64_t Kp, const void* B, int64_t ldb, const float* b_scale, void* C, int64_t ldc, const adt_gemm_epilogue* ep) {
   GemmI8Args g{};
-  g.A = static_cast<const signed char*>(A); g.lda = lda; g.a_scale = a_scale;
   g.B = static_cast<const signed char*>(B); g.ldb = ldb; g.b_scale = b_scale;
   g.C = C; g.ldc = ldc; g.bias = ep->bias; g.residual = static_cast<const float*>(ep->residual); g.ld_res = ep->ld_res; g.res_row_mod = ep->res_row_mod;
   g.aux = static_cast<unsigned short*>(ep->aux_bf16_out); g.ld_aux = ep->ld_aux;
-  g.M = static_cast<int>(M); g.N = static_cast<int>(N); g.K = static_cast<int>(K); g.act = ep->act;
+  g.M = static_cast<int>(M); g.N = static_cast<int>(N); g.K = static_cast<int>(Kp); g.act = ep->act;
   auto ok = [](const void* p, int64_t ld, int elem) { return !p || (aligned16(p) && (ld * elem) % 16 == 0); };
   g.vec = (N % 8) == 0 && ok(C, ldc, ep->out_fp32 ? 4 : 2) && ok(g.bias, 4, 4) && ok(b_scale, 4, 4) && ok(g.residual, g.ld_res, 4) && ok(g.aux, g.ld_aux, 2);
-  const int64_t tm = (M + 127) / 128, tn = (N + 127) / 128;
-  if (tm * tn > (1LL << 31) - 1) return set_error(ADT_ESHAPE, "adt_gemm_i8: too many tiles");
-  const auto fn = ep->out_fp32 ? gemm_i8_kernel<true> : gemm_i8_kernel<false>;
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(tm * tn)), dim3(256), kI8Lds, static_cast<hipStream_t>(stream), g, static_cast<int>(tm), static_cast<int>(tn));
+  return g;
+}
+template <bool kOut32, int kMT, int kX>
+static int launch_i8_skinny(const GemmI8Args& g, const LinearX& lx, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((g.N + 15) / 16), static_cast<unsigned>((g.M + 16 * kMT - 1) / (16 * kMT)));
+  hipLaunchKernelGGL((gemm_i8_skinny_kernel<kOut32, kMT, kX>), grid, dim3(64 * kI8SkinnyWaves), 0, st, g, lx);
   ADT_HIP_TRY(hipGetLastError());
   return ADT_OK;
+}
+template <bool kOut32>
+static int launch_i8(const GemmI8Args& g, hipStream_t st) {
+  typedef void (*Fn)(GemmI8Args, int, int);
+  typedef void (*BigFn)(GemmI8Args, int, int, int);
+  static const Fn fns[4] = {gemm_i8_kernel<kOut32, 0>, gemm_i8_kernel<kOut32, 1>, gemm_i8_kernel<kOut32, 2>, gemm_i8_kernel<kOut32, 3>};
+  static const BigFn big[4] = {gemm_i8_256_kernel<kOut32, 0>, gemm_i8_256_kernel<kOut32, 1>, gemm_i8_256_kernel<kOut32, 2>, gemm_i8_256_kernel<kOut32, 3>};
+  int n_cu = 0;
+  if (int rc = device_cu_count(&n_cu)) return rc;
+  const bool extra = g.residual || g.aux;
+  int form = kI8Any;
+  if (g.vec) form = g.act == 0 ? (extra ? kI8Residual : kI8Plain) : (g.act == 1 && !extra ? kI8Gelu : kI8Any);
+  const int64_t tm = (g.M + 127) / 128, tn = (g.N + 127) / 128, bm = (g.M + 255) / 256, bn = (g.N + 255) / 256;
+  // Few tokens: while its workgroups of 64 tokens x 16 channels are at most two per CU, the kernel that asks for everything at once wins
+  // (768 deep, us here / with 128 x 128 tiles: 64 x 1400 4.3 / 7.6, 256 x 768 4.3 / 7.7, 256 x 2304 8.3 / 7.9, 512 x 768 6.3 / 7.7, 1024 x 768 8.6 / 7.8).
+  if (static_cast<int64_t>((g.M + 63) / 64) * ((g.N + 15) / 16) <= 2 * n_cu && (g.M + 15) / 16 <= 65535) {
+    if (g.M <= 16) return launch_i8_skinny<kOut32, 1, kXInt8>(g, LinearX{}, st);
+    if (g.M <= 32) return launch_i8_skinny<kOut32, 2, kXInt8>(g, LinearX{}, st);
+    return launch_i8_skinny<kOut32, 4, kXInt8>(g, LinearX{}, st);
+  }
+  // 256 x 256 tiles run one per CU and twice as efficiently, but in whole rounds: a round of them costs 1.6 of 128 x 128 ones at two per CU (us with
+  // 256 / 128: 4096 x 2304 x 768 16.4 / 18.9, 7747 x 768 x 768 14.6 / 11.2, 8192 x 2304 x 768 29.4 / 29.3, 16384 x 2304 x 768 43.6 / 53.1,
+  // 63104 x 2304 x 768 140 / 240, 2048 x 4096 x 4096 43.8 / 45.1, 4096^3 55.2 / 85.3).
+  if (8 * ((bm * bn + n_cu - 1) / n_cu) <= 5 * ((tm * tn + 2 * n_cu - 1) / (2 * n_cu))) {
+    const BigFn fn = big[(g.K & 127) ? kI8Any : form];
+    ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, kI8BigLds));
+    const int64_t wgs = bm * bn < n_cu ? bm * bn : n_cu;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(wgs)), dim3(512), kI8BigLds, st, g, static_cast<int>(bm), static_cast<int>(bn), 3);
+  } else {
+    if (tm * tn > (1LL << 31) - 1) return set_error(ADT_ESHAPE, "adt_gemm_i8: too many tiles");
+    hipLaunchKernelGGL(fns[form], dim3(static_cast<unsigned>(tm * tn)), dim3(256), kI8Lds, st, g, static_cast<int>(tm), static_cast<int>(tn));
+  }
+  ADT_HIP_TRY(hipGetLastError());
+  return ADT_OK;
+}
+}  // namespace adt
+
+extern "C" int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const float* a_scale, const void* B, int64_t ldb,
+                           const float* b_scale, void* C, int64_t ldc, const adt_gemm_epilogue* ep, void* stream) {
+  if (!A || !a_scale) return set_error(ADT_EINVAL, "adt_gemm_i8: null pointer");
+  if (int rc = gemm_i8_check("adt_gemm_i8", M, N, K, B, ldb, b_scale, C, ldc, ep)) return rc;
+  if (K & 15) return set_error(ADT_ESHAPE, "adt_gemm_i8: K must be a multiple of 16");
+  if (lda < K || (lda & 15) || !aligned16(A)) return set_error(ADT_EINVAL, "adt_gemm_i8: operand rows are 16-byte aligned and hold K");
+  if (M == 0 || N == 0) return ADT_OK;
+  GemmI8Args g = gemm_i8_args(M, N, K, B, ldb, b_scale, C, ldc, ep);
+  g.A = static_cast<const signed char*>(A); g.lda = lda; g.a_scale = a_scale;
+  return ep->out_fp32 ? launch_i8<true>(g, static_cast<hipStream_t>(stream)) : launch_i8<false>(g, static_cast<hipStream_t>(stream));
+}
+
+// Rows quantised inside the product: up to 16 of them, as long as a workgroup holds them in its registers (us in one launch / in two: 1 x 2304 x 768 3.8 / 5.2,
+// 16 x 2304 x 768 4.1 / 5.6, 16 x 768 x 2048 6.2 / 7.0, 16 x 4096 x 4096 13.4 / 11.7).
+static bool linear_i8_fused(int64_t M, int64_t K) { return M <= 16 && K <= 64 * adt::kI8SkinnyDepth * adt::kI8SkinnyWaves; }
+
+extern "C" size_t adt_linear_i8_workspace_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || linear_i8_fused(M, K)) return 0;
+  return static_cast<size_t>(M) * ((K + 15) / 16 * 16) + static_cast<size_t>(M) * 4;
+}
+
+extern "C" int adt_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int32_t x_fp32, int64_t ldx, const void* W, int64_t ldw, const float* w_scale,
+                             void* C, int64_t ldc, const adt_gemm_epilogue* ep, void* ws, size_t ws_bytes, void* stream) {
+  if (!x) return set_error(ADT_EINVAL, "adt_linear_i8: null pointer");
+  if (int rc = gemm_i8_check("adt_linear_i8", M, N, K, W, ldw, w_scale, C, ldc, ep)) return rc;
+  if (ldx < K) return set_error(ADT_EINVAL, "adt_linear_i8: rows of x hold K elements");
+  if (M == 0 || N == 0) return ADT_OK;
+  const int64_t Kp = (K + 15) / 16 * 16;
+  GemmI8Args g = gemm_i8_args(M, N, Kp, W, ldw, w_scale, C, ldc, ep);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (linear_i8_fused(M, K)) {
+    const LinearX lx{x, static_cast<long>(ldx), static_cast<int>(K), aligned16(x) && (ldx * (x_fp32 ? 4 : 2)) % 16 == 0};
+    if (ep->out_fp32) return x_fp32 ? launch_i8_skinny<true, 1, kXF32>(g, lx, st) : launch_i8_skinny<true, 1, kXBf16>(g, lx, st);
+    return x_fp32 ? launch_i8_skinny<false, 1, kXF32>(g, lx, st) : launch_i8_skinny<false, 1, kXBf16>(g, lx, st);
+  }
+  if (!ws || ws_bytes < adt_linear_i8_workspace_bytes(M, K) || !aligned16(ws)) return set_error(ADT_EINVAL, "adt_linear_i8: workspace too small or not 16-byte aligned");
+  float* scale = reinterpret_cast<float*>(static_cast<char*>(ws) + M * Kp);
+  if (int rc = adt_quant_rows_i8(x, x_fp32, ldx, M, K, ws, Kp, scale, stream)) return rc;
+  g.A = static_cast<const signed char*>(ws); g.lda = Kp; g.a_scale = scale;
+  return ep->out_fp32 ? launch_i8<true>(g, st) : launch_i8<false>(g, st);
 }

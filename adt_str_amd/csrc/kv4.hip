@@ -12,11 +12,12 @@
 //   V: channel 16 b + i and the eight tokens 4 u + {0..3}, 16 + 4 u + {0..3} are one dword, number ((b / 4) 64 + 16 u + i) 4 + (b & 3): a lane's
 //      (i = lane & 15, u = lane >> 4) 16-byte pieces are its operands of four products over 32 tokens; the token order is the one in which a lane
 //      holds the scores.
-//   A dword's element j is at bits 4 (j / 2) + 16 (j & 1): (w << 3), (w >> 1), (w >> 5), (w >> 9), masked to 0x00780078 and joined with 0x41804180,
-//   are four pairs of the bf16 numbers 16 + c.
+//   A dword's element j is at bits 4 (j / 2) + 16 (j & 1): w, w >> 4, w >> 8 and w >> 12, masked to 0x000f000f and joined with 0x43004300, are four pairs
+//   of the bf16 numbers 128 + c.
 //   A parameter dword is the bf16 scale (low half) and the bf16 minimum (high half).
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdio>
 
 #include "adt_common.h"
@@ -66,114 +67,194 @@ __device__ __forceinline__ KvRange kv_range(const KvArgs& a, int b) {
 }
 
 // ------------------------------------------------------------------------------------ append
-// One wave per (32-token tile, head, sequence) and side (K or V).  A lane holds eight channels of a row: D/8 lanes per row, 512 / D rows at a
-// time; eight lanes share a group, whose extrema are three exchanges.  (x - lo) / s is a correctly rounded quotient: q0 = d y, y = 1 / s,
-// corrected by the exact remainder fma(-q0, s, d).
-// The K codes of a lane are one dword of the record.  The V codes go through LDS as bytes [token][channel] and leave as the dwords of
-// eight tokens; a tile that is not written whole keeps its other tokens' codes (the wave is the only writer of its record half).
+// One wave per (32-token tile, head, sequence) and side (K or V).  A lane holds eight channels of a row, D/8 lanes a row, and goes through the
+// tokens whose codes share a dword of the V record, 4 u + {0..3} and 16 + 4 u + {0..3} (at 64 channels one half of them): its eight channels' dwords
+// then fill up in its registers, and the K codes of a row are one dword per lane anyway.  All rows are requested before the first is used.
+//   extrema: bf16 numbers, sign-folded, order like 16-bit integers (NaNs at the ends, so that they and infinities show in the range), two per
+//            instruction; eight lanes share a group and exchange in the DPP network
+//   codes: (x - lo) / s is a correctly rounded quotient, q0 = d y, y = 1 / s, corrected by the exact remainder fma(-q0, s, d); rounding to the integer is the
+//            addition of 2^23, whose low half is then the code.  It is 15 at most: s is (hi - lo) / 15 to 2^-9.
+// The V dwords pass through LDS once to leave as 16-byte pieces; a tile that is not written whole keeps its other tokens' codes (the wave is
+// the only writer of its record half).
+// Bound: vector instructions, 110 per eight values, about the time of the memory traffic (63104 rows of 768, K and V).
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned kv_fold(unsigned w) {             // two bf16 numbers <-> 16-bit integers of the same order
+  const s16x2 x = __builtin_bit_cast(s16x2, w);
+  return w ^ (__builtin_bit_cast(unsigned, x >> static_cast<short>(15)) & 0x7fff7fffu);
+}
+__device__ __forceinline__ unsigned kv_pk_min(unsigned a, unsigned b) {
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+}
+__device__ __forceinline__ unsigned kv_pk_max(unsigned a, unsigned b) {
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+}
+template <int kCtrl>
+__device__ __forceinline__ unsigned kv_dpp(unsigned v) { return __builtin_amdgcn_update_dpp(v, v, kCtrl, 0xf, 0xf, false); }
+__device__ __forceinline__ unsigned kv_halves(unsigned hi, unsigned lo) { return __builtin_amdgcn_perm(hi, lo, 0x05040100u); }      // lo & 0xffff | hi << 16
+
 template <int D>
 __global__ __launch_bounds__(128) void kv4_append_kernel(KvArgs a) {
   using R = KvRec<D>;
-  constexpr int kLanes = D / 8, kRows = 64 / kLanes;   // lanes per row, rows per pass
-  __shared__ unsigned char vb[kKvTile][D + 4];
-  const int lane = threadIdx.x & 63, side = threadIdx.x >> 6;      // side 0: K, 1: V
+  constexpr int kLanes = D / 8, kJ = D == 128 ? 8 : 4;             // lanes per row, rows per lane
+  __shared__ __attribute__((aligned(16))) unsigned vl[D / 64][4][72];      // [piece][u][16 channels x 4 blocks + 8: the four u on different banks]
+  const int lane = threadIdx.x & 63, side = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);      // side 0: K, 1: V
   const int b = blockIdx.z, h = blockIdx.y;
   const KvRange r = kv_range(a, b);
   const int tile = (r.lo >> 5) + static_cast<int>(blockIdx.x);
   if (tile * kKvTile >= r.hi || r.lo >= r.hi) return;  // block-uniform
   unsigned char* rec = a.cache + (static_cast<long>(b * a.H + h) * a.tiles + tile) * R::kBytes;
   const int t0 = max(r.lo - tile * kKvTile, 0), t1 = min(r.hi - tile * kKvTile, kKvTile);      // tokens of the tile that are written
-  const int c8 = lane % kLanes, sub = lane / kLanes;
+  const int c8 = lane % kLanes, sub = lane / kLanes, u = sub & 3, half = sub >> 2;            // (half: 64 channels only)
   const unsigned short* src = side ? a.v : a.k;
   const long ld = side ? a.ldv : a.ldk;
-  unsigned* par = reinterpret_cast<unsigned*>(rec + (side ? R::kVp : R::kKp)) + (c8 >> 3) * kKvTile;
-  for (int t = sub; t < kKvTile; t += kRows) {
-    const bool live = t >= t0 && t < t1;
-    const int tt = live ? t : t0;                      // (every lane takes part in the exchanges)
-    const unsigned short* p = src + (static_cast<long>(b) * a.n + (tile * kKvTile + tt - r.first)) * ld + h * D + 8 * c8;
-    float x[8];
-    if (((reinterpret_cast<uintptr_t>(src) & 15) | (ld & 7)) == 0) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+  const unsigned short* row0 = src + (static_cast<long>(b) * a.n + (tile * kKvTile - r.first)) * ld + h * D + 8 * c8;      // (of token 0, which need not exist)
+  const bool vec = ((reinterpret_cast<uintptr_t>(src) & 15) | (ld & 7)) == 0;
+  auto token_of = [&](int j) { return 16 * (D == 128 ? j >> 2 : half) + 4 * u + (j & 3); };
+  unsigned any = 0;                                    // bit j: some lane's row j is written (uniform)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(w[j] << 16); x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+  for (int t = 0; t < kKvTile; ++t)
+    if (t >= t0 && t < t1) any |= 1u << (D == 128 ? (t & 3) + 4 * (t >> 4) : t & 3);
+  u32x4 raw[kJ];
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    if (!(any >> j & 1u)) continue;
+    const int t = token_of(j);
+    const unsigned short* p = row0 + (t >= t0 && t < t1 ? t : t0) * ld;      // (every lane takes part in the exchanges)
+    if (vec) {
+      raw[j] = *reinterpret_cast<const u32x4*>(p);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = kv_bf2f(p[j]);
+      for (int i = 0; i < 4; ++i) raw[j][i] = p[2 * i] | static_cast<unsigned>(p[2 * i + 1]) << 16;
     }
-    float lo = x[0], hi = x[0];
-    bool bad = false;
+  }
+  unsigned* par = reinterpret_cast<unsigned*>(rec + (side ? R::kVp : R::kKp)) + (c8 >> 3) * kKvTile;
+  unsigned vw[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};   // channel i's dword
+  unsigned even[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo = fminf(lo, x[j]); hi = fmaxf(hi, x[j]);
-      bad |= !(fabsf(x[j]) < INFINITY);
-    }
-    unsigned bb = bad ? 1u : 0u;
+  for (int j = 0; j < kJ; ++j) {
+    unsigned bits[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    if (any >> j & 1u) {
+      const int t = token_of(j);
+      const bool live = t >= t0 && t < t1;
+      unsigned f[4];
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o)); hi = fmaxf(hi, __shfl_xor(hi, o)); bb |= __shfl_xor(bb, o); }
-    const float range = hi - lo;
-    bad = bb != 0 || !(range < INFINITY);
-    const unsigned sb = kv_f2bf(fmaxf(range / 15.0f, kKvTiny));
-    const float s = kv_bf2f(sb), y = 1.0f / s;
-    unsigned code[8];
+      for (int i = 0; i < 4; ++i) f[i] = kv_fold(raw[j][i]);
+      unsigned lo2 = kv_pk_min(kv_pk_min(f[0], f[1]), kv_pk_min(f[2], f[3])), hi2 = kv_pk_max(kv_pk_max(f[0], f[1]), kv_pk_max(f[2], f[3]));
+      lo2 = kv_pk_min(lo2, kv_dpp<0xB1>(lo2)); hi2 = kv_pk_max(hi2, kv_dpp<0xB1>(hi2));          // lane ^ 1
+      lo2 = kv_pk_min(lo2, kv_dpp<0x4E>(lo2)); hi2 = kv_pk_max(hi2, kv_dpp<0x4E>(hi2));          // lane ^ 2
+      lo2 = kv_pk_min(lo2, kv_dpp<0x141>(lo2)); hi2 = kv_pk_max(hi2, kv_dpp<0x141>(hi2));        // mirrored in eight lanes: the other four
+      lo2 = kv_pk_min(lo2, lo2 >> 16);                 // (the low half)
+      hi2 = kv_pk_max(hi2, hi2 << 16);                 // (the high half)
+      const unsigned both = kv_fold((lo2 & 0xffffu) | (hi2 & 0xffff0000u));
+      const float lo = kv_bf2f(both & 0xffffu), hi = __uint_as_float(both & 0xffff0000u);
+      const float range = hi - lo;
+      const bool bad = !(range < INFINITY);
+      constexpr float y15 = 1.0f / 15.0f;
+      const float s0 = range * y15;                    // a correctly rounded range / 15, as the codes are
+      const unsigned sb = kv_f2bf(fmaxf(fmaf(fmaf(-s0, 15.0f, range), y15, s0), kKvTiny));
+      const float s = kv_bf2f(sb);
+      const float y0 = __builtin_amdgcn_rcpf(s), y = fmaf(fmaf(-s, y0, 1.0f), y0, y0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = x[j] - lo;
-      const float q0 = d * y;
-      const float q = fmaf(fmaf(-q0, s, d), y, q0);
-      code[j] = bad ? 0u : __float_as_uint(fminf(q, 15.0f) + 12582912.0f) & 15u;
-    }
-    if (live) {
-      if ((c8 & 7) == 0) par[t] = bad ? 0x7fc07fc0u : (sb | (__float_as_uint(lo) & 0xffff0000u));
-      if (side == 0) {
-        unsigned w = 0;
+      for (int i = 0; i < 8; ++i) {
+        const float x = i & 1 ? __uint_as_float(raw[j][i >> 1] & 0xffff0000u) : __uint_as_float(raw[j][i >> 1] << 16);
+        const float d = x - lo;
+        const float q0 = d * y;
+        bits[i] = __float_as_uint(fmaf(fmaf(-q0, s, d), y, q0) + 8388608.0f);
+      }
+      if (__builtin_amdgcn_ballot_w64(bad || !live) != 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w |= code[j] << (4 * (j >> 1) + 16 * (j & 1));
-        // channels 8 c8 .. + 7 = 32 g + 8 u with g = c8 / 4, u = c8 & 3
+        for (int i = 0; i < 8; ++i) bits[i] = bad || !live ? 0u : bits[i];
+      }
+      if (live && (c8 & 7) == 0) par[t] = bad ? 0x7fc07fc0u : (sb | both << 16);
+      if (side == 0 && live) {
+        const unsigned w = kv_halves(bits[1], bits[0]) | kv_halves(bits[3], bits[2]) << 4 | kv_halves(bits[5], bits[4]) << 8 | kv_halves(bits[7], bits[6]) << 12;
+        // channels 8 c8 .. + 7 = 32 g + 8 v with g = c8 / 4, v = c8 & 3
         reinterpret_cast<unsigned*>(rec + t * R::kRow)[(D / 32) * (c8 & 3) + (c8 >> 2)] = w;
+      }
+    }
+    if (side) {                                        // rows 2 k and 2 k + 1: nibble k of the dword's halves
+      if (j & 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vw[i] |= kv_halves(bits[i], even[i]) << (4 * (j >> 1));
       } else {
-        *reinterpret_cast<unsigned*>(&vb[t][8 * c8]) = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
-        *reinterpret_cast<unsigned*>(&vb[t][8 * c8 + 4]) = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) even[i] = bits[i];
       }
     }
   }
   if (side == 0) return;
-  __builtin_amdgcn_wave_barrier();                     // one wave wrote vb and reads it back: its LDS operations are in order
-  unsigned* vw = reinterpret_cast<unsigned*>(rec + R::kV);
-  const int i = lane & 15, u = lane >> 4;
+  unsigned keep = 0;                                   // of lane (channel lane & 15, u = lane >> 4) of the pieces: the nibbles of tokens that stay
 #pragma unroll
-  for (int blk = 0; blk < D / 16; ++blk) {
-    unsigned w = 0, mask = 0;
+  for (int j = 0; j < 8; ++j) {
+    const int t = (j < 4 ? 0 : 16) + 4 * (lane >> 4) + (j & 3);
+    if (t < t0 || t >= t1) keep |= 15u << (4 * (j >> 1) + 16 * (j & 1));
+  }
+  if constexpr (D == 64) {                             // the other half's tokens: lane ^ 32; each of the two writes four channels
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int t = (j < 4 ? 0 : 16) + 4 * u + (j & 3), sh = 4 * (j >> 1) + 16 * (j & 1);
-      if (t >= t0 && t < t1) { w |= static_cast<unsigned>(vb[t][16 * blk + i]) << sh; mask |= 15u << sh; }
+    for (int i = 0; i < 8; ++i) {
+      if (half) vw[i] <<= 8;
+      vw[i] |= __shfl_xor(vw[i], 32);
     }
-    unsigned* p = vw + ((blk >> 2) * 64 + lane) * 4 + (blk & 3);
-    if (mask == 0xffffffffu) *p = w;
-    else if (mask) *p = (*p & ~mask) | w;
+  }
+  // channel 8 c8 + i: block c8 / 2, its channel 8 (c8 & 1) + i
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (D == 128 || (i >> 2) == half) vl[c8 >> 3][u][(8 * (c8 & 1) + i) * 4 + ((c8 >> 1) & 3)] = vw[i];
+  __builtin_amdgcn_wave_barrier();                     // one wave wrote vl and reads it back: its LDS operations are in order
+  u32x4* out = reinterpret_cast<u32x4*>(rec + R::kV);
+#pragma unroll
+  for (int piece = 0; piece < D / 64; ++piece) {
+    u32x4 w = *reinterpret_cast<const u32x4*>(&vl[piece][lane >> 4][(lane & 15) * 4]);
+    u32x4* p = out + piece * 64 + lane;
+    if (keep == 0u) {
+      *p = w;
+    } else if (keep != 0xffffffffu) {
+      const u32x4 old = *p;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] |= old[k] & keep;
+      *p = w;
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------ read
-// Rows i < count of every sequence as the numbers they stand for (bf16 or fp32), the other rows of the output zeros.
+// Rows i < count of every sequence as the numbers they stand for (bf16 or fp32), the other rows of the output zeros.  One wave per 32 output
+// rows and side; where those lie in a tile (or two) a wave holds the tile's V codes in LDS, as they come.
 template <int D, bool k32>
 __global__ __launch_bounds__(128) void kv4_read_kernel(KvArgs a) {
   using R = KvRec<D>;
   constexpr int kLanes = D / 8, kRows = 64 / kLanes;
+  __shared__ unsigned vl[2][32 * D / 8];               // the V codes of the one or two tiles that the 32 rows lie in
   const int lane = threadIdx.x & 63, side = threadIdx.x >> 6;
   const int b = blockIdx.z, h = blockIdx.y;
   const KvRange r = kv_range(a, b);
   const int c8 = lane % kLanes, sub = lane / kLanes;
   void* out = side ? a.vo : a.ko;
   const long ld = side ? a.ldvo : a.ldko;
+  const int i0 = blockIdx.x * kKvTile;
+  const long first = static_cast<long>(r.first) + i0;                  // the position of row i0
+  const long lo = max(first, static_cast<long>(r.lo)), hi = min(first + kKvTile, static_cast<long>(r.hi));
+  const unsigned char* recs = a.cache + static_cast<long>(b * a.H + h) * a.tiles * R::kBytes;
+  const int tile0 = static_cast<int>(lo >> 5);
+  if (side && lo < hi) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (tile0 + k > static_cast<int>((hi - 1) >> 5)) break;
+      const u32x4* p = reinterpret_cast<const u32x4*>(recs + static_cast<long>(tile0 + k) * R::kBytes + R::kV);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) reinterpret_cast<u32x4*>(vl[k])[i * 64 + lane] = p[i * 64 + lane];
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
   for (int t = sub; t < kKvTile; t += kRows) {
-    const int i = blockIdx.x * kKvTile + t;
+    const int i = i0 + t;
     if (i >= a.n) break;
-    const long pos = static_cast<long>(r.first) + i;
+    const long pos = first + t;
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (pos >= r.lo && pos < r.hi) {
-      const unsigned char* rec = a.cache + (static_cast<long>(b * a.H + h) * a.tiles + (pos >> 5)) * R::kBytes;
-      const int tt = pos & 31;
+    if (pos >= lo && pos < hi) {
+      const int tile = static_cast<int>(pos >> 5), tt = static_cast<int>(pos & 31);
+      const unsigned char* rec = recs + static_cast<long>(tile) * R::kBytes;
       const unsigned par = reinterpret_cast<const unsigned*>(rec + (side ? R::kVp : R::kKp))[(c8 >> 3) * kKvTile + tt];
       const float s = kv_bf2f(par & 0xffffu), m = __uint_as_float(par & 0xffff0000u);
       if (side == 0) {
@@ -182,7 +263,7 @@ __global__ __launch_bounds__(128) void kv4_read_kernel(KvArgs a) {
         for (int j = 0; j < 8; ++j) x[j] = static_cast<float>((w >> (4 * (j >> 1) + 16 * (j & 1))) & 15u) * s + m;
       } else {
         const int u = (tt & 15) >> 2, j8 = (tt & 3) + (tt & 16 ? 4 : 0), sh = 4 * (j8 >> 1) + 16 * (j8 & 1);
-        const unsigned* vw = reinterpret_cast<const unsigned*>(rec + R::kV);
+        const unsigned* vw = vl[tile - tile0];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int d = 8 * c8 + j, blk = d >> 4;
@@ -203,26 +284,30 @@ __global__ __launch_bounds__(128) void kv4_read_kernel(KvArgs a) {
 }
 
 // ------------------------------------------------------------------------------------ attention
-// A workgroup = four waves on one (sequence, K/V head, block of 16 rows, span of tiles); a row is a (query position, query head of the group)
-// pair, row = position * group + head.  A wave takes every fourth tile of the span:
+// A workgroup = kW waves on one (sequence, K/V head, block of 16 rows, span of tiles); a row is a (query position, query head of the group)
+// pair, row = position * group + head.  A wave takes every kW-th tile of the span:
 //   scores  S[token][row] = sum_g s_g (K codes . q)_g + m_g (sum of q)_g    two 16 x 16 x 32 bf16 products per group and 16 tokens; the codes enter as
-//           16 + c, and the accumulator starts at -16 (sum of q)_g, so it ends at the sum of c q: q and the codes are exact in bf16, the sums fp32
+//           128 + c, and the accumulator starts at -128 (sum of q)_g, so it ends at the sum of c q: q and the codes are exact in bf16, the sums fp32
 //   softmax over the tokens: a lane holds eight tokens of one row; one running maximum per row, raised only when a score exceeds it by more
 //           than 2^8 (the probabilities are then at most 2^8 and the sums stay exact to fp32), so the cross-lane exchange is rare
-//   output  O[row][channel] += (p s_g) (16 + c)   the weight p s_g goes in as two bf16 numbers, upper and lower half (2^-17 of it is lost);
-//           p (m_g - 16 s_g) is added up per row and group in fp32 on the side.
+//   output  O[row][channel] += (p s_g) (128 + c) - 128 (p s_g)    the weight p s_g goes in as two bf16 numbers, upper and lower half (2^-17 of it is
+//           lost), and the subtrahend is a product of the same two with ones, so that the offset costs no accuracy; p m_g is added up per
+//           row and group in fp32 on the side.
 // The waves' (max, sum, O) join through LDS; with more than one span per head they go to the workspace and a second kernel joins them.
+// Bound: the instructions beside the products (340 per wave and tile at D = 128, 56 + 56 of them unpacking codes), about 8 TB/s of cache on the
+// whole chip, then the memory.  The next tile's K (V) is requested as soon as this tile's K (V) is used up.
 struct KvAttnArgs {
   const unsigned short* q; long ldq; bool qvec;        // qvec: 16-byte loads of q
   const unsigned char* cache; int B, Hk, group, cap, tiles;
   const int* key_len;
   unsigned short* out; long ldo; float* lse;
-  int q_len, causal; float sl2;                        // scale * log2 e
+  int q_len, causal; float sl2; bool negate;           // |scale| * log2 e, and q enters negated for a negative scale
   int rows, row_blocks, spans, span_tiles;             // rows = q_len * group
   float* part;                                         // spans > 1: [B][Hk][rows][spans][D + 2]
 };
 constexpr float kKvNegBig = -3.0e38f;               // below every score: the running maximum of a row that has seen no token
 constexpr float kKvThr = 8.0f;
+constexpr int kKvMaxSpans = 64;
 
 __device__ __forceinline__ float kv_max_over_groups(float v) {      // over the four lanes that share lane & 15
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -233,120 +318,152 @@ __device__ __forceinline__ float kv_sum_over_groups(float v) {
   return v + __shfl_xor(v, 32);
 }
 union KvFrag { unsigned u[4]; bf16x8 v; };
-__device__ __forceinline__ KvFrag kv_unpack(unsigned w) {            // eight codes -> the bf16 numbers 16 + c
+// eight codes -> the bf16 numbers 128 + c; mask and bits are 0x000f000f and 0x43004300 in registers (one instruction takes one literal at most)
+__device__ __forceinline__ KvFrag kv_unpack(unsigned w, unsigned mask, unsigned bits) {
   KvFrag f;
-  f.u[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
-  f.u[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-  f.u[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-  f.u[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f.u[i] = ((w >> (4 * i)) & mask) | bits;
   return f;
 }
+__device__ __forceinline__ float kv_scale_of(unsigned par) { return __uint_as_float(par << 16); }
+__device__ __forceinline__ float kv_min_of(unsigned par) { return __uint_as_float(par & 0xffff0000u); }
 
-template <int D>
-__global__ __launch_bounds__(256) void attn_kv4_kernel(KvAttnArgs a) {
+template <int D, int kW>
+__global__ __launch_bounds__(64 * kW, kW == 4 ? 3 : 1) void attn_kv4_kernel(KvAttnArgs a, int n_max) {      // n_max = min(16, rows)
   using R = KvRec<D>;
-  constexpr int kG = R::kG, kNB = D / 16, kPieces = D / 64;          // V pieces (16 bytes) per lane and tile; K: D/64 dword pairs per 16 tokens
-  __shared__ float sm[4][16], sl[4][16], sc[4][kG][16];
-  __shared__ float so[4][16][D + 4];
+  constexpr int kG = R::kG, kNB = D / 16, kPieces = D / 64;          // V pieces (16 bytes) per lane and tile
+  constexpr int kPitch = D + 4;
+  static_assert(64 * kW >= 2 * D, "a thread per sixteen bytes of q");
+  extern __shared__ __attribute__((aligned(16))) float so[];         // [kW][n_max][kPitch] at the end; the rows of q at the start
+  __shared__ float sm[kW][16], sl[kW][16], sc[kW][kG][16];
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, u = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int id = blockIdx.x;
   const int span = id % a.spans; id /= a.spans;
   const int rb = id % a.row_blocks; id /= a.row_blocks;
   const int hk = id % a.Hk, b = id / a.Hk;
+  // ---- everything the first tile needs is asked for at once: the length, this block's rows of q (sixteen bytes per thread, two-byte loads where
+  // the rows are not aligned), the tile itself (the span's last one at most, whatever the length is)
   int klen = a.key_len ? a.key_len[b] : a.cap;
+  u32x4 qw = {0u, 0u, 0u, 0u};
+  if (tid < 2 * D) {
+    const int row = rb * 16 + tid / (D / 8), c = 8 * (tid % (D / 8));
+    if (row < a.rows) {
+      const unsigned short* p = a.q + (static_cast<long>(b) * a.q_len + row / a.group) * a.ldq + (hk * a.group + row % a.group) * D + c;
+      if (a.qvec) {
+        qw = *reinterpret_cast<const u32x4*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qw[j] = p[2 * j] | static_cast<unsigned>(p[2 * j + 1]) << 16;
+      }
+    }
+  }
+  const unsigned char* const base = a.cache + static_cast<long>(b * a.Hk + hk) * a.tiles * R::kBytes;
+  unsigned kw[2][D / 32];
+  u32x4 vw[kPieces], kp[2][kG], vp[2][kG];
+  auto load_k = [&](int t) __attribute__((always_inline)) {
+    const unsigned char* rec = base + static_cast<long>(t) * R::kBytes;
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb) {
+      const unsigned* p = reinterpret_cast<const unsigned*>(rec + (16 * hb + li) * R::kRow + 4 * (D / 32) * u);
+      if constexpr (D == 128) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) kw[hb][s] = w[s];
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        kw[hb][0] = w.x; kw[hb][1] = w.y;
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g) kp[hb][g] = *reinterpret_cast<const u32x4*>(rec + R::kKp + (g * kKvTile + 16 * hb + 4 * u) * 4);
+    }
+  };
+  auto load_v = [&](int t) __attribute__((always_inline)) {
+    const unsigned char* rec = base + static_cast<long>(t) * R::kBytes;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) vw[i] = *reinterpret_cast<const u32x4*>(rec + R::kV + (i * 64 + lane) * 16);
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+      for (int g = 0; g < kG; ++g) vp[hb][g] = *reinterpret_cast<const u32x4*>(rec + R::kVp + (g * kKvTile + 16 * hb + 4 * u) * 4);
+  };
+  int tile = span * a.span_tiles + wave;
+  load_k(min(tile, a.tiles - 1));
+  load_v(min(tile, a.tiles - 1));
   klen = klen < 0 ? 0 : (klen > a.cap ? a.cap : klen);
-  // this lane's row (as a column of the score product)
-  const int row = rb * 16 + li;
-  const bool live = row < a.rows;
-  const int qi = live ? row / a.group : 0, qh = live ? row % a.group : 0;
-  const unsigned short* qp = a.q + (static_cast<long>(b) * a.q_len + qi) * a.ldq + (hk * a.group + qh) * D + 8 * u;
+  const int qlast = min(rb * 16 + 15, a.rows - 1) / a.group;
+  const int most = a.causal ? klen - (a.q_len - 1 - qlast) : klen;   // the tokens that some row of this block sees
+  const int tile_end = min((max(most, 0) + kKvTile - 1) / kKvTile, (span + 1) * a.span_tiles);
+
+  unsigned short* const ql = reinterpret_cast<unsigned short*>(so);  // [16][D + 8]
+  constexpr int kQPitch = D + 8;
+  if (a.negate) qw ^= 0x80008000u;
+  if (tid < 2 * D) *reinterpret_cast<u32x4*>(ql + (tid / (D / 8)) * kQPitch + 8 * (tid % (D / 8))) = qw;
+  __syncthreads();
   KvFrag qf[D / 32];
   float qs[kG];
 #pragma unroll
   for (int g = 0; g < kG; ++g) qs[g] = 0.f;
 #pragma unroll
   for (int s = 0; s < D / 32; ++s) {
-    if (a.qvec) {
-      const u32x4 w = live ? *reinterpret_cast<const u32x4*>(qp + 32 * s) : u32x4{0u, 0u, 0u, 0u};
+    const u32x4 w = *reinterpret_cast<const u32x4*>(ql + li * kQPitch + 32 * s + 8 * u);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) qf[s].u[j] = w[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned lo = live ? qp[32 * s + 2 * j] : 0u, hi = live ? qp[32 * s + 2 * j + 1] : 0u;
-        qf[s].u[j] = lo | hi << 16;
-      }
+    for (int j = 0; j < 4; ++j) {
+      qf[s].u[j] = w[j];
+      qs[s / 2] += kv_scale_of(w[j]) + kv_min_of(w[j]);              // (the two halves as numbers)
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) qs[s / 2] += kv_bf2f(qf[s].u[j] & 0xffffu) + __uint_as_float(qf[s].u[j] & 0xffff0000u);
   }
 #pragma unroll
   for (int g = 0; g < kG; ++g) qs[g] = kv_sum_over_groups(qs[g]);
-  const int limit = a.causal ? klen - (a.q_len - 1 - qi) : klen;      // tokens [0, limit) are this row's
-  // the tiles any row of this block can see
-  const int qlast = min(rb * 16 + 15, a.rows - 1) / a.group;
-  const int most = a.causal ? klen - (a.q_len - 1 - qlast) : klen;
-  const int tile_end = min((max(most, 0) + kKvTile - 1) / kKvTile, (span + 1) * a.span_tiles);
+  __syncthreads();                                                   // ql becomes so
+  // this lane's row (as a column of the score product) sees the tokens [0, limit)
+  const int limit = a.causal ? klen - (a.q_len - 1 - min(rb * 16 + li, a.rows - 1) / a.group) : klen;
+  const int least = a.causal ? klen - (a.q_len - 1) : klen;
 
+  unsigned mask = 0x000f000fu, bits = 0x43004300u;
+  asm volatile("" : "+v"(mask), "+s"(bits));
   float m = kKvNegBig, l = 0.f, cb[kG];
-  f32x4 o[kNB];
+  f32x4 o[kNB], os[kG];
 #pragma unroll
   for (int i = 0; i < kNB; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int g = 0; g < kG; ++g) cb[g] = 0.f;
+  for (int g = 0; g < kG; ++g) { cb[g] = 0.f; os[g] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  KvFrag ones;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ones.u[j] = 0x3f803f80u;
 
-  const unsigned char* base = a.cache + static_cast<long>(b * a.Hk + hk) * a.tiles * R::kBytes;
-  for (int tile = span * a.span_tiles + wave; tile < tile_end; tile += 4) {
-    const unsigned char* rec = base + static_cast<long>(tile) * R::kBytes;
-    unsigned kw[2][D / 32];
-    u32x4 vw[kPieces], kp[2][kG], vp[2][kG];
-#pragma unroll
-    for (int hb = 0; hb < 2; ++hb) {
-      const unsigned* p = reinterpret_cast<const unsigned*>(rec + (16 * hb + li) * R::kRow) + (D / 32) * u;
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) kw[hb][s] = p[s];
-#pragma unroll
-      for (int g = 0; g < kG; ++g) {
-        kp[hb][g] = *reinterpret_cast<const u32x4*>(rec + R::kKp + (g * kKvTile + 16 * hb + 4 * u) * 4);
-        vp[hb][g] = *reinterpret_cast<const u32x4*>(rec + R::kVp + (g * kKvTile + 16 * hb + 4 * u) * 4);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) vw[i] = *reinterpret_cast<const u32x4*>(rec + R::kV + (i * 64 + lane) * 16);
-    // ---- scores (log2 units)
+  for (; tile < tile_end; tile += kW) {
+    const int next = min(tile + kW, tile_end - 1);                   // (past the end: a tile that is there, for nothing)
     float z[8];
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
       f32x4 acc[kG];
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        const float c0 = -16.0f * qs[g];
+        const float c0 = -128.0f * qs[g];
         acc[g] = f32x4{c0, c0, c0, c0};
 #pragma unroll
-        for (int s = 2 * g; s < 2 * g + 2; ++s) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv_unpack(kw[hb][s]).v, qf[s].v, acc[g], 0, 0, 0);
+        for (int s = 2 * g; s < 2 * g + 2; ++s) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv_unpack(kw[hb][s], mask, bits).v, qf[s].v, acc[g], 0, 0, 0);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float t = 0.f;
+        float t = kv_min_of(kp[hb][0][r]) * qs[0];
+        t = fmaf(kv_scale_of(kp[hb][0][r]), acc[0][r], t);
 #pragma unroll
-        for (int g = 0; g < kG; ++g) t += __uint_as_float(kp[hb][g][r] << 16) * acc[g][r] + __uint_as_float(kp[hb][g][r] & 0xffff0000u) * qs[g];
-        z[4 * hb + r] = t * a.sl2;
+        for (int g = 1; g < kG; ++g) t = fmaf(kv_scale_of(kp[hb][g][r]), acc[g][r], fmaf(kv_min_of(kp[hb][g][r]), qs[g], t));
+        z[4 * hb + r] = t;
       }
     }
+    load_k(next);
     const int key0 = tile * kKvTile + 4 * u;
-    const bool edge = (tile + 1) * kKvTile > (a.causal ? klen - (a.q_len - 1) : klen);      // block-uniform: some row does not see all of it
+    const bool edge = (tile + 1) * kKvTile > least;                  // block-uniform: some row does not see all of the tile
     if (edge) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = key0 + (j < 4 ? j : 12 + j);
-        if (key >= limit) z[j] = kKvNegBig;
-      }
+      for (int j = 0; j < 8; ++j)
+        if (key0 + (j < 4 ? j : 12 + j) >= limit) z[j] = kKvNegBig;
     }
-    float mx = z[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, z[j]);
-    if (__ballot(mx > m + kKvThr) != 0) {
+    float mx = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))) * a.sl2;
+    if (__builtin_amdgcn_ballot_w64(mx > m + kKvThr) != 0) {
       const float m_new = fmaxf(m, kv_max_over_groups(mx));
       const float alpha = __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
@@ -355,44 +472,49 @@ __global__ __launch_bounds__(256) void attn_kv4_kernel(KvAttnArgs a) {
       for (int g = 0; g < kG; ++g) cb[g] *= alpha;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float ar = __shfl(alpha, 4 * u + r);                    // the output's rows are 4 u + r
+        const float ar = __shfl(alpha, 4 * u + r);                   // the output's rows are 4 u + r
 #pragma unroll
         for (int i = 0; i < kNB; ++i) o[i][r] *= ar;
+#pragma unroll
+        for (int g = 0; g < kG; ++g) os[g][r] *= ar;
       }
     }
     float p[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(z[j] - m);
-      if (edge && key0 + (j < 4 ? j : 12 + j) >= limit) p[j] = 0.f;
-      l += p[j];
+    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(z[j], a.sl2, -m));
+    if (edge) {                                                      // what a row does not see may be anything
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (key0 + (j < 4 ? j : 12 + j) >= limit) {
+          p[j] = 0.f;
+#pragma unroll
+          for (int g = 0; g < kG; ++g) vp[j >> 2][g][j & 3] = 0u;
+        }
     }
-    // ---- output
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l += p[j];
 #pragma unroll
     for (int g = 0; g < kG; ++g) {
       KvFrag hi, lo;
-      float ps[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        unsigned par = vp[j >> 2][g][j & 3];
-        if (edge && key0 + (j < 4 ? j : 12 + j) >= limit) par = 0;    // what a row does not see may be anything
-        const float s = __uint_as_float(par << 16), mn = __uint_as_float(par & 0xffff0000u);
-        ps[j] = p[j] * s;
-        cb[g] += p[j] * mn - 16.0f * ps[j];
-      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const unsigned a0 = __float_as_uint(ps[2 * j]) & 0xffff0000u, a1 = __float_as_uint(ps[2 * j + 1]) & 0xffff0000u;
-        hi.u[j] = a0 >> 16 | a1;
-        lo.u[j] = kv_pack_bf2(ps[2 * j] - __uint_as_float(a0), ps[2 * j + 1] - __uint_as_float(a1));
+        const unsigned p0 = vp[j >> 1][g][(2 * j) & 3], p1 = vp[j >> 1][g][(2 * j + 1) & 3];
+        const float w0 = p[2 * j] * kv_scale_of(p0), w1 = p[2 * j + 1] * kv_scale_of(p1);
+        cb[g] = fmaf(p[2 * j], kv_min_of(p0), cb[g]);
+        cb[g] = fmaf(p[2 * j + 1], kv_min_of(p1), cb[g]);
+        hi.u[j] = __builtin_amdgcn_perm(__float_as_uint(w1), __float_as_uint(w0), 0x07060302u);
+        lo.u[j] = kv_pack_bf2(w0 - kv_min_of(__float_as_uint(w0)), w1 - kv_min_of(__float_as_uint(w1)));
       }
+      os[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi.v, ones.v, os[g], 0, 0, 0);
+      os[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo.v, ones.v, os[g], 0, 0, 0);
 #pragma unroll
       for (int i = 4 * g; i < 4 * g + 4; ++i) {
-        const KvFrag vf = kv_unpack(vw[i >> 2][i & 3]);
+        const KvFrag vf = kv_unpack(vw[i >> 2][i & 3], mask, bits);
         o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi.v, vf.v, o[i], 0, 0, 0);
         o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo.v, vf.v, o[i], 0, 0, 0);
       }
     }
+    load_v(next);
   }
   // ---- the waves join
   l = kv_sum_over_groups(l);
@@ -404,25 +526,30 @@ __global__ __launch_bounds__(256) void attn_kv4_kernel(KvAttnArgs a) {
     for (int g = 0; g < kG; ++g) sc[wave][g][li] = cb[g];
   }
 #pragma unroll
-  for (int i = 0; i < kNB; ++i)
+  for (int r = 0; r < 4; ++r) {
+    if (4 * u + r >= n_max) continue;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) so[wave][4 * u + r][16 * i + li] = o[i][r];
+    for (int i = 0; i < kNB; ++i) so[(wave * n_max + 4 * u + r) * kPitch + 16 * i + li] = fmaf(-128.0f, os[i / 4][r], o[i][r]);
+  }
   __syncthreads();
   const int n_rows = min(16, a.rows - rb * 16);
-  for (int e = tid; e < n_rows * D; e += 256) {
+  for (int e = tid; e < n_rows * D; e += 64 * kW) {
     const int rr = e / D, d = e % D;
-    const float mm = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr]));
+    float mm = sm[0][rr];
+#pragma unroll
+    for (int w = 1; w < kW; ++w) mm = fmaxf(mm, sm[w][rr]);
     float lt = 0.f, ot = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kW; ++w) {
       const float f = __builtin_amdgcn_exp2f(sm[w][rr] - mm);
-      lt += f * sl[w][rr];
-      ot += f * (so[w][rr][d] + sc[w][d >> 6][rr]);
+      lt = fmaf(f, sl[w][rr], lt);
+      ot = fmaf(f, so[(w * n_max + rr) * kPitch + d] + sc[w][d >> 6][rr], ot);
     }
     const int orow = rb * 16 + rr, oi = orow / a.group, oh = hk * a.group + orow % a.group;
+    const bool any = lt > 0.f || lt != lt;
     if (a.spans == 1) {
-      a.out[(static_cast<long>(b) * a.q_len + oi) * a.ldo + oh * D + d] = static_cast<unsigned short>(kv_f2bf(lt > 0.f || lt != lt ? ot / lt : 0.f));
-      if (d == 0 && a.lse) a.lse[(static_cast<long>(b) * (a.Hk * a.group) + oh) * a.q_len + oi] = lt > 0.f || lt != lt ? (mm + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+      a.out[(static_cast<long>(b) * a.q_len + oi) * a.ldo + oh * D + d] = static_cast<unsigned short>(kv_f2bf(any ? ot / lt : 0.f));
+      if (d == 0 && a.lse) a.lse[(static_cast<long>(b) * (a.Hk * a.group) + oh) * a.q_len + oi] = any ? (mm + log2f(lt)) * 0.6931471805599453f : -INFINITY;
     } else {
       float* part = a.part + (((static_cast<long>(b) * a.Hk + hk) * a.rows + orow) * a.spans + span) * (D + 2);
       part[d] = ot;
@@ -431,26 +558,26 @@ __global__ __launch_bounds__(256) void attn_kv4_kernel(KvAttnArgs a) {
   }
 }
 
+// One row per workgroup, a thread per channel: lane s weighs span s (at most 64 of them), the spans' outputs are then independent loads.
 template <int D>
-__global__ __launch_bounds__(64) void attn_kv4_join_kernel(KvAttnArgs a) {
+__global__ __launch_bounds__(D) void attn_kv4_join_kernel(KvAttnArgs a) {
   const int orow = blockIdx.x % a.rows, bh = blockIdx.x / a.rows, hk = bh % a.Hk, b = bh / a.Hk;
+  const int lane = threadIdx.x & 63;
   const float* part = a.part + (static_cast<long>(bh) * a.rows + orow) * a.spans * (D + 2);
-  float mm = kKvNegBig;
-  for (int s = 0; s < a.spans; ++s) mm = fmaxf(mm, part[s * (D + 2) + D]);
-  float lt = 0.f, ot[D / 64];
+  float ms = kKvNegBig, ls = 0.f;
+  if (lane < a.spans) { ms = part[lane * (D + 2) + D]; ls = part[lane * (D + 2) + D + 1]; }
+  float mm = ms;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) ot[i] = 0.f;
-  for (int s = 0; s < a.spans; ++s) {
-    const float f = __builtin_amdgcn_exp2f(part[s * (D + 2) + D] - mm);
-    lt += f * part[s * (D + 2) + D + 1];
+  for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+  const float f = __builtin_amdgcn_exp2f(ms - mm);
+  float lt = f * ls, ot = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) ot[i] += f * part[s * (D + 2) + 64 * i + threadIdx.x];
-  }
+  for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o);
+#pragma unroll 8
+  for (int s = 0; s < a.spans; ++s) ot = fmaf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s)), part[s * (D + 2) + threadIdx.x], ot);
   const int oi = orow / a.group, oh = hk * a.group + orow % a.group;
   const bool any = lt > 0.f || lt != lt;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    a.out[(static_cast<long>(b) * a.q_len + oi) * a.ldo + oh * D + 64 * i + threadIdx.x] = static_cast<unsigned short>(kv_f2bf(any ? ot[i] / lt : 0.f));
+  a.out[(static_cast<long>(b) * a.q_len + oi) * a.ldo + oh * D + threadIdx.x] = static_cast<unsigned short>(kv_f2bf(any ? ot / lt : 0.f));
   if (threadIdx.x == 0 && a.lse) a.lse[(static_cast<long>(b) * (a.Hk * a.group) + oh) * a.q_len + oi] = any ? (mm + log2f(lt)) * 0.6931471805599453f : -INFINITY;
 }
 
@@ -481,8 +608,11 @@ static int kv_rows_check(const char* who, int64_t B, int64_t H, int64_t D, const
   snprintf(msg, sizeof(msg), "%s: %s", who, what);
   return set_error(ADT_EINVAL, msg);
 }
-struct KvPlan { int rows, row_blocks, tiles, spans, span_tiles; };
-// Spans per head: a workgroup's four waves want two tiles each at least, and below three workgroups per CU the chip is not full.
+struct KvPlan { int rows, row_blocks, tiles, spans, span_tiles, waves; };
+// A wave takes 0.7 us per tile when it has its SIMD to itself (420 instructions), a call 5 us around its tiles and 2 us more for the join of spans.  With
+// at most a workgroup per CU: eight waves each, and spans until there is one per CU or a wave has one tile (us with waves / spans: 6 heads x 986
+// positions 8/4 8.1, 8/1 9.4, 4/1 10.5; 64 x 32000 8/4 67.8, 8/1 207, 4/8 67.6; 120 x 3001, 64 channels, 8/2 13.1, 4/1 17.5).  With more: four waves,
+// three workgroups fit a CU, and spans only where less than half of that is in use (384 x 986 4/1 17.9, 4/2 17.7, 8/1 18.9; 1536 x 986 43.4, 49.6, 52.4).
 static int kv_plan(const adt_attn_kv4_desc* d, KvPlan* p) {
   int n_cu = 256;
   (void)device_cu_count(&n_cu);
@@ -490,11 +620,23 @@ static int kv_plan(const adt_attn_kv4_desc* d, KvPlan* p) {
   p->row_blocks = (p->rows + 15) / 16;
   p->tiles = (d->capacity + kKvTile - 1) / kKvTile;
   const long wgs = static_cast<long>(d->batch) * d->kv_heads * p->row_blocks;
-  long want = wgs > 0 ? (3L * n_cu + wgs - 1) / wgs : 1;
-  const long most = (p->tiles + 7) / 8;
-  want = want < 1 ? 1 : (want > most ? most : want);
+  p->waves = wgs <= n_cu ? 8 : 4;
+  long want = wgs <= 0 ? 1 : (p->waves == 8 ? (n_cu + wgs - 1) / wgs : 5L * n_cu / (2 * wgs));
+  const long most = (p->tiles + p->waves - 1) / p->waves;
+  want = want > most ? most : want;
+  want = want < 1 ? 1 : (want > kKvMaxSpans ? kKvMaxSpans : want);
   p->span_tiles = static_cast<int>((p->tiles + want - 1) / want);
   p->spans = (p->tiles + p->span_tiles - 1) / p->span_tiles;
+  return ADT_OK;
+}
+template <int D, int kW>
+static int launch_attn_kv4(const KvAttnArgs& a, unsigned wgs, hipStream_t st) {
+  const int n_max = a.rows < 16 ? a.rows : 16;
+  const int q_bytes = 16 * (D + 8) * 2, o_bytes = kW * n_max * (D + 4) * 4, lds = o_bytes > q_bytes ? o_bytes : q_bytes;
+  if (lds > 64 * 1024 - 4096)
+    ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(attn_kv4_kernel<D, kW>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL((attn_kv4_kernel<D, kW>), dim3(wgs), dim3(64 * kW), lds, st, a, n_max);
+  ADT_HIP_TRY(hipGetLastError());
   return ADT_OK;
 }
 static int kv_desc_check(const adt_attn_kv4_desc* d, const void* cache) {
@@ -571,16 +713,15 @@ extern "C" int adt_attn_kv4(const adt_attn_kv4_desc* d, const void* q, const voi
   a.q = static_cast<const unsigned short*>(q); a.ldq = d->ldq; a.qvec = aligned16(q) && d->ldq % 8 == 0;
   a.cache = static_cast<const unsigned char*>(cache); a.B = d->batch; a.Hk = d->kv_heads; a.group = d->heads / d->kv_heads; a.cap = d->capacity;
   a.tiles = p.tiles; a.key_len = d->key_len; a.out = static_cast<unsigned short*>(o); a.ldo = d->ldo; a.lse = lse;
-  a.q_len = d->q_len; a.causal = d->causal; a.sl2 = d->scale * 1.4426950408889634f;
+  a.q_len = d->q_len; a.causal = d->causal; a.sl2 = fabsf(d->scale) * 1.4426950408889634f; a.negate = d->scale < 0.f;
   a.rows = p.rows; a.row_blocks = p.row_blocks; a.spans = p.spans; a.span_tiles = p.span_tiles; a.part = static_cast<float*>(ws);
   const int64_t wgs = static_cast<int64_t>(d->batch) * d->kv_heads * p.row_blocks * p.spans, joins = static_cast<int64_t>(d->batch) * d->kv_heads * p.rows;
   if (wgs > (1LL << 31) - 1 || joins > (1LL << 31) - 1) return set_error(ADT_ESHAPE, "adt_attn_kv4: too many workgroups");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (d->head_dim == 128) hipLaunchKernelGGL(attn_kv4_kernel<128>, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(attn_kv4_kernel<64>, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, st, a);
-  ADT_HIP_TRY(hipGetLastError());
+  const auto launch = d->head_dim == 128 ? (p.waves == 8 ? launch_attn_kv4<128, 8> : launch_attn_kv4<128, 4>) : (p.waves == 8 ? launch_attn_kv4<64, 8> : launch_attn_kv4<64, 4>);
+  if (int rc = launch(a, static_cast<unsigned>(wgs), st)) return rc;
   if (p.spans > 1) {
-    if (d->head_dim == 128) hipLaunchKernelGGL(attn_kv4_join_kernel<128>, dim3(static_cast<unsigned>(joins)), dim3(64), 0, st, a);
+    if (d->head_dim == 128) hipLaunchKernelGGL(attn_kv4_join_kernel<128>, dim3(static_cast<unsigned>(joins)), dim3(128), 0, st, a);
     else hipLaunchKernelGGL(attn_kv4_join_kernel<64>, dim3(static_cast<unsigned>(joins)), dim3(64), 0, st, a);
     ADT_HIP_TRY(hipGetLastError());
   }

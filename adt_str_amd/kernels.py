@@ -641,34 +641,29 @@ def check_attn_bwd() -> None:
 
 
 # ---- serving in few bits: 8-bit-integer linear layers (K16) ------------------------------------------------------------------------
-class _on_device:
-    """The launches inside go to the current stream of the tensors' own device, whichever device is current; all tensors must share it."""
-    __slots__ = ("index", "back")
-
-    def __init__(self, *tensors):
-        dev = None
-        for t in tensors:
-            if t is None:
-                continue
-            if not t.is_cuda:
-                raise RuntimeError("adt_str_amd kernels take GPU tensors only (there is no CPU path)")
+def _device_of(*tensors) -> int:
+    """Index of the one device that the tensors (None allowed) lie on."""
+    dev = -1
+    for t in tensors:
+        if t is not None:
             i = t.get_device()
-            if dev is None:
+            if i < 0:
+                raise RuntimeError("adt_str_amd kernels take GPU tensors only (there is no CPU path)")
+            if i != dev:
+                if dev >= 0:
+                    raise RuntimeError(f"tensors of one call lie on different devices ({dev} and {i})")
                 dev = i
-            elif i != dev:
-                raise RuntimeError(f"tensors of one call lie on different devices ({dev} and {i})")
-        self.index = dev
+    return dev
 
-    def __enter__(self):
-        self.back = torch.cuda.current_device()
-        if self.back != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
 
-    def __exit__(self, exc_type, exc, tb):
-        if self.back != self.index:
-            torch.cuda.set_device(self.back)
-        return False
+def _launch(dev: int, name: str, *args) -> None:
+    """``_ffi.call`` with the current stream of device ``dev`` as the last argument, whichever device is current."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)      # (torch.cuda.current_stream(dev).cuda_stream without the object: a microsecond)
+    if dev == torch.cuda.current_device():
+        _ffi.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _ffi.call(name, *args, stream)
 
 
 def quant_rows_i8(x: torch.Tensor):
@@ -677,11 +672,11 @@ def quant_rows_i8(x: torch.Tensor):
     or a NaN gets the scale NaN.  Serves activations (scale per token) and weights ``[N, K]`` (scale per output channel) alike."""
     assert x.dtype in (torch.bfloat16, torch.float32) and x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1)
     M, K = x.shape
-    with _on_device(x) as stream:
-        q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-        scale = torch.empty(M, dtype=torch.float32, device=x.device)
-        _ffi.call("adt_quant_rows_i8", x.data_ptr() if M else 16, int(x.dtype == torch.float32), x.stride(0) if M > 1 else max(x.stride(0), K), M, K,
-                  q.data_ptr() if M else 16, q.shape[1], scale.data_ptr() if M else 16, stream)
+    dev = _device_of(x)
+    q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    if M:
+        _launch(dev, "adt_quant_rows_i8", x.data_ptr(), x.dtype == torch.float32, max(x.stride(0), K), M, K, q.data_ptr(), q.shape[1], scale.data_ptr())
     return q, scale
 
 
@@ -713,22 +708,36 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     assert K > 0 and K % 16 == 0 and a.stride(1) == 1 and b.stride(1) == 1
     for s, n in ((a_scale, M), (b_scale, N)):
         assert s.dtype == torch.float32 and s.dim() == 1 and s.numel() == n and s.is_contiguous()
-    with _on_device(a, a_scale, b, b_scale, out, bias, residual, aux_bf16_out) as stream:
-        if out is None:
-            out = torch.empty((M, N), dtype=out_dtype, device=a.device)
-        ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
-        if M and N:
-            _ffi.call("adt_gemm_i8", M, N, K, a.data_ptr(), max(a.stride(0), K), a_scale.data_ptr(), b.data_ptr(), max(b.stride(0), K), b_scale.data_ptr(),
-                      out.data_ptr(), max(out.stride(0), N), C.byref(ep), stream)
+    dev = _device_of(a, a_scale, b, b_scale, out, bias, residual, aux_bf16_out)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
+    if M and N:
+        _launch(dev, "adt_gemm_i8", M, N, K, a.data_ptr(), max(a.stride(0), K), a_scale.data_ptr(), b.data_ptr(), max(b.stride(0), K), b_scale.data_ptr(),
+                out.data_ptr(), max(out.stride(0), N), C.byref(ep))
     return out
 
 
-def linear_i8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, **kw) -> torch.Tensor:
-    """``x [M, K]`` (bf16 / fp32) through a linear layer whose weights are int8 with one scale per output channel (``w8, w_scale =
-    quant_rows_i8(weight)``): the rows are quantised (``quant_rows_i8``) and multiplied (``gemm_i8``, whose keyword arguments this takes)."""
-    assert x.dim() == 2 and w8.dim() == 2 and w8.shape[1] == (x.shape[1] + 15) // 16 * 16, (x.shape, w8.shape)
-    q, scale = quant_rows_i8(x)
-    return gemm_i8(q, scale, w8, w_scale, **kw)
+def linear_i8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, *, out: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16,
+              bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, res_row_mod: int = 0, act: int = 0,
+              aux_bf16_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x [M, K]`` (bf16 / fp32, row-strided views allowed) through a linear layer whose weights are int8 with one scale per output channel
+    (``w8, w_scale = quant_rows_i8(weight)``): the rows are quantised (``quant_rows_i8``) and multiplied (``gemm_i8``) in one call
+    (``adt_linear_i8``), up to 16 rows of 2048 in one launch; the same bits as the two."""
+    assert x.dtype in (torch.bfloat16, torch.float32) and x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1)
+    assert w8.dtype == torch.int8 and w8.dim() == 2 and w8.stride(1) == 1 and w8.shape[1] == (x.shape[1] + 15) // 16 * 16, (x.shape, w8.shape)
+    (M, K), N = x.shape, w8.shape[0]
+    assert w_scale.dtype == torch.float32 and w_scale.dim() == 1 and w_scale.numel() == N and w_scale.is_contiguous()
+    dev = _device_of(x, w8, w_scale, out, bias, residual, aux_bf16_out)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
+    if M and N:
+        nb = _ffi.load().adt_linear_i8_workspace_bytes(M, K)
+        ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None      # (from the allocator: a captured call gets its graph's own)
+        _launch(dev, "adt_linear_i8", M, N, K, x.data_ptr(), x.dtype == torch.float32, max(x.stride(0), K), w8.data_ptr(), max(w8.stride(0), w8.shape[1]),
+                w_scale.data_ptr(), out.data_ptr(), max(out.stride(0), N), C.byref(ep), ws.data_ptr() if nb else None, nb)
+    return out
 
 
 # ---- serving in few bits: the 4-bit K/V cache (K17) --------------------------------------------------------------------------------
@@ -770,9 +779,9 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, end: Optional[
     assert k.shape[0] % cache.batch == 0, (k.shape, cache.batch)
     n = k.shape[0] // cache.batch
     width = _kv4_rows(cache, end, count, k, v, n)
-    with _on_device(cache.data, k, v, end, count) as stream:
-        _ffi.call("adt_kv4_append", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity, k.data_ptr(), max(k.stride(0), width),
-                  v.data_ptr(), max(v.stride(0), width), n, end.data_ptr() if end is not None else None, count.data_ptr() if count is not None else None, stream)
+    _launch(_device_of(cache.data, k, v, end, count), "adt_kv4_append", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity,
+            k.data_ptr(), max(k.stride(0), width), v.data_ptr(), max(v.stride(0), width), n, end.data_ptr() if end is not None else None,
+            count.data_ptr() if count is not None else None)
 
 
 def kv4_read(cache: KV4Cache, end: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None, n: Optional[int] = None, out_dtype=torch.bfloat16):
@@ -782,12 +791,12 @@ def kv4_read(cache: KV4Cache, end: Optional[torch.Tensor] = None, count: Optiona
     n = cache.capacity if n is None else int(n)
     assert n >= 0
     width = cache.kv_heads * cache.head_dim
-    with _on_device(cache.data, end, count) as stream:
-        k, v = (torch.empty((cache.batch * n, width), dtype=out_dtype, device=cache.data.device) for _ in range(2))
-        if cache.batch and n:
-            _kv4_rows(cache, end, count, k, v, n)
-            _ffi.call("adt_kv4_read", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity, k.data_ptr(), width, v.data_ptr(), width,
-                      int(out_dtype == torch.float32), n, end.data_ptr() if end is not None else None, count.data_ptr() if count is not None else None, stream)
+    dev = _device_of(cache.data, end, count)
+    k, v = (torch.empty((cache.batch * n, width), dtype=out_dtype, device=cache.data.device) for _ in range(2))
+    if cache.batch and n:
+        _kv4_rows(cache, end, count, k, v, n)
+        _launch(dev, "adt_kv4_read", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity, k.data_ptr(), width, v.data_ptr(), width,
+                out_dtype == torch.float32, n, end.data_ptr() if end is not None else None, count.data_ptr() if count is not None else None)
     return k, v
 
 
@@ -802,16 +811,17 @@ def attn_kv4(q: torch.Tensor, cache: KV4Cache, key_len: Optional[torch.Tensor] =
     assert q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q_len > 0 and heads > 0 and heads % cache.kv_heads == 0
     assert q.shape[0] == rows and q.shape[1] >= width, (q.shape, rows, width)
     assert key_len is None or (key_len.dtype == torch.int32 and key_len.dim() == 1 and key_len.numel() == cache.batch and key_len.is_contiguous())
-    with _on_device(q, cache.data, key_len, out) as stream:
-        if out is None:
-            out = torch.empty((rows, width), dtype=torch.bfloat16, device=q.device)
-        assert out.dtype == torch.bfloat16 and out.shape == (rows, width) and out.stride(1) == 1
-        lse = torch.empty((cache.batch, heads, q_len), dtype=torch.float32, device=q.device) if want_lse else None
-        if rows:
-            d = _ffi.AttnKv4Desc(cache.batch, heads, cache.kv_heads, cache.head_dim, q_len, cache.capacity, int(causal), float(scale),
-                                 max(q.stride(0), width), max(out.stride(0), width), key_len.data_ptr() if key_len is not None else None)
-            nb = _ffi.load().adt_attn_kv4_workspace_bytes(C.byref(d))
-            ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None       # (from the allocator: a captured call gets its graph's own)
-            _ffi.call("adt_attn_kv4", C.byref(d), q.data_ptr(), cache.data.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
-                      ws.data_ptr() if nb else None, nb, stream)
+    dev = _device_of(q, cache.data, key_len, out)
+    if out is None:
+        out = torch.empty((rows, width), dtype=torch.bfloat16, device=q.device)
+    assert out.dtype == torch.bfloat16 and out.shape == (rows, width) and out.stride(1) == 1
+    lse = torch.empty((cache.batch, heads, q_len), dtype=torch.float32, device=q.device) if want_lse else None
+    if rows:
+        d = _ffi.AttnKv4Desc(cache.batch, heads, cache.kv_heads, cache.head_dim, q_len, cache.capacity, causal, scale,
+                             max(q.stride(0), width), max(out.stride(0), width), key_len.data_ptr() if key_len is not None else None)
+        ref = C.byref(d)
+        nb = _ffi.load().adt_attn_kv4_workspace_bytes(ref)
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None       # (from the allocator: a captured call gets its graph's own)
+        _launch(dev, "adt_attn_kv4", ref, q.data_ptr(), cache.data.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
+                ws.data_ptr() if nb else None, nb)
     return (out, lse) if want_lse else out

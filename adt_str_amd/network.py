@@ -282,8 +282,9 @@ class _Engine:
             return K.gemm(x, part(lin.w16), bias=bias, **kw)
         if kw.get("drop", 0) is None:                     # inference: no dropout site is on
             kw = {k: v for k, v in kw.items() if k not in ("drop", "drop_after_residual")}
-        q, scale = x if isinstance(x, tuple) else K.quant_rows_i8(x)
-        return K.gemm_i8(q, scale, part(lin.w8), part(lin.w_scale), bias=bias, **kw)
+        if isinstance(x, tuple):
+            return K.gemm_i8(*x, part(lin.w8), part(lin.w_scale), bias=bias, **kw)
+        return K.linear_i8(x, part(lin.w8), part(lin.w_scale), bias=bias, **kw)
 
     def _quant(self, x):
         return K.quant_rows_i8(x) if self.int8 else x
