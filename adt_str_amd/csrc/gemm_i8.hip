@@ -9,7 +9,6 @@
 
 #include <algorithm>
 #include <cstdio>
-#include <cstdlib>
 
 #include "adt_common.h"
 
@@ -38,7 +37,7 @@ __device__ __forceinline__ float i8_gelu(float x) {
 }
 
 // ------------------------------------------------------------------------------------ row quantiser
-// One wave per row.  The codes are those of real arithmetic: with e the exponent of a, n = x 127 2^-e is exact for bf16 x (and carried with
+// 16 to 256 lanes per row.  The codes are those of real arithmetic: with e the exponent of a, n = x 127 2^-e is exact for bf16 x (and carried with
 // its rounding error for fp32 x), b = a 2^-e lies in [1, 2), and n / b is formed as r0 = n y, y = 1 / b, corrected by the exact remainder
 // fma(-r0, b, n): a correctly rounded quotient, so that x = a / 2 is 63.5 and not a neighbour of it.  Rounding to the integer is the
 // addition of 1.5 2^23, whose low byte is then the code.
@@ -99,7 +98,14 @@ __device__ __forceinline__ void load8(const QuantArgs& a, long row, int k, bool 
 template <int kLanes>
 __device__ __forceinline__ unsigned lanes_max_u32(unsigned v) {
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) { const unsigned t = __shfl_xor(v, o); v = t > v ? t : v; }
+  for (int o = (kLanes < 64 ? kLanes : 64) / 2; o > 0; o >>= 1) { const unsigned t = __shfl_xor(v, o); v = t > v ? t : v; }
+  if constexpr (kLanes == 256) {                 // the workgroup's four waves share a row
+    __shared__ unsigned part[4];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v = part[w] > v ? part[w] : v;
+  }
   return v;
 }
 __device__ __forceinline__ unsigned widest8(const float (&v)[8], unsigned mx) {
@@ -164,8 +170,13 @@ struct GemmI8Args {
   void* C; long ldc;
   const float* bias; const float* residual; long ld_res; int res_row_mod; unsigned short* aux; long ld_aux;
   int M, N, K, act;
-  bool vec;                     // N % 8 == 0 and every row of C, bias, b_scale, residual and aux 16-byte aligned
+  bool stream;                  // the rows of C are whole 128-byte lines
 };
+// Rows of the outputs and the residual begin wherever the caller's strides put them, so their 16-byte pieces are typed by their elements' alignment;
+// the hardware takes wide accesses there: 17297 x 2602 x 1190 in bf16 takes 70 us, one element at a time it took 150.
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 __device__ __forceinline__ int w_row_bf16(int j, int i) { return 32 * (j >> 1) + 8 * (i >> 2) + 4 * (j & 1) + (i & 3); }
 
 // What a call's epilogue is made of, as far as it is known when the kernel is compiled: everything at run time costs the 256 x 256 kernel 80 KB of
@@ -173,49 +184,61 @@ __device__ __forceinline__ int w_row_bf16(int j, int i) { return 32 * (j >> 1) +
 __device__ __forceinline__ const float* i8_residual(const GemmI8Args& g, long m, int n) {
   return g.residual + (g.res_row_mod ? static_cast<unsigned>(m) % static_cast<unsigned>(g.res_row_mod) : m) * g.ld_res + n;
 }
-constexpr int kI8Plain = 0, kI8Gelu = 1, kI8Residual = 2, kI8Any = 3;      // rows as GemmI8Args::vec, and no residual / copy except kI8Residual; kI8Any: whatever the call says
-template <bool kOut32, int kN>
-__device__ __forceinline__ void i8_store(const GemmI8Args& g, long m, int n, const int (&acc)[kN], float as, const float (&bs)[kN], const float (&bias)[kN]) {
-  float z[kN];
-  const float* res = g.residual ? i8_residual(g, m, n) : nullptr;
+constexpr int kI8Plain = 0, kI8Gelu = 1, kI8Residual = 2, kI8Any = 3;      // no activation / GELU, and no residual / copy; residual and / or copy, no activation; whatever the call says
+__device__ __forceinline__ f32x4 i8_residual4(const GemmI8Args& g, long m, int n) {
+  const float* r = i8_residual(g, m, n);
+  if (n + 4 <= g.N) return *reinterpret_cast<const f32x4_any*>(r);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < kN; ++e) {
-    z[e] = static_cast<float>(acc[e]) * as * bs[e] + bias[e];
-    if (g.act == 1) z[e] = i8_gelu(z[e]);
-    else if (g.act == 2) z[e] = fmaxf(z[e], 0.f);
-  }
-  if (g.vec && n + kN <= g.N) {
-    if (res) {
-#pragma unroll
-      for (int e = 0; e < kN; e += 4) {
-        const f32x4 r = *reinterpret_cast<const f32x4*>(res + e);
-        z[e] += r[0]; z[e + 1] += r[1]; z[e + 2] += r[2]; z[e + 3] += r[3];
-      }
-    }
-    if (kOut32) {
-      float* c = static_cast<float*>(g.C) + m * g.ldc + n;
-#pragma unroll
-      for (int e = 0; e < kN; e += 4) *reinterpret_cast<f32x4*>(c + e) = f32x4{z[e], z[e + 1], z[e + 2], z[e + 3]};
-    }
-    unsigned p[kN / 2];
-#pragma unroll
-    for (int e = 0; e < kN / 2; ++e) p[e] = i8_pack_bf2(z[2 * e], z[2 * e + 1]);
-    unsigned short* h = kOut32 ? g.aux : static_cast<unsigned short*>(g.C);
-    const long ldh = kOut32 ? g.ld_aux : g.ldc;
-    if (!kOut32 || h) {
-      if constexpr (kN == 8) *reinterpret_cast<u32x4*>(h + m * ldh + n) = u32x4{p[0], p[1], p[2], p[3]};
-      else *reinterpret_cast<uint2*>(h + m * ldh + n) = make_uint2(p[0], p[1]);
+  for (int e = 0; e < 4; ++e)
+    if (n + e < g.N) v[e] = r[e];
+  return v;
+}
+// A piece of a row, channels n ..: eight bf16 results or four fp32 ones.  Where rows are whole 128-byte lines the 256 x 256 kernel's leave
+// nontemporal (63104 x 2304 x 768: 132 / 155 us with and without, fp32 169 / 210; 16384 x 2312 x 768, where they are not, 52.6 / 42.0, fp32 96 / 59).
+template <bool kStream>
+__device__ __forceinline__ void i8_put_bf16(unsigned short* row, int n, int n_end, u32x4 v, bool stream) {
+  if (n + 8 <= n_end) {
+    u32x4_any* c = reinterpret_cast<u32x4_any*>(row + n);
+    if (kStream && stream) {                     // (the empty statements keep the two stores two: joined, they lose the hint)
+      asm volatile("" ::: "memory");
+      __builtin_nontemporal_store(v, c);
+      asm volatile("" ::: "memory");
+    } else {
+      *c = v;
     }
     return;
   }
 #pragma unroll
-  for (int e = 0; e < kN; ++e) {
-    if (n + e >= g.N) continue;
-    const float v = res ? z[e] + res[e] : z[e];
-    if (kOut32) static_cast<float*>(g.C)[m * g.ldc + n + e] = v;
-    else static_cast<unsigned short*>(g.C)[m * g.ldc + n + e] = i8_f2bf(v);
-    if (kOut32 && g.aux) g.aux[m * g.ld_aux + n + e] = i8_f2bf(v);
+  for (int e = 0; e < 8; ++e)
+    if (n + e < n_end) row[n + e] = static_cast<unsigned short>(v[e >> 1] >> (16 * (e & 1)));
+}
+template <bool kStream>
+__device__ __forceinline__ void i8_put_f32(float* row, int n, int n_end, f32x4 v, bool stream) {
+  if (n + 4 <= n_end) {
+    f32x4_any* c = reinterpret_cast<f32x4_any*>(row + n);
+    if (kStream && stream) {                     // (the empty statements keep the two stores two: joined, they lose the hint)
+      asm volatile("" ::: "memory");
+      __builtin_nontemporal_store(v, c);
+      asm volatile("" ::: "memory");
+    } else {
+      *c = v;
+    }
+    return;
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < n_end) row[n + e] = v[e];
+}
+__device__ __forceinline__ void i8_put_copy(unsigned short* row, int n, int n_end, f32x4 v) {      // four bf16 results
+  const unsigned lo = i8_pack_bf2(v[0], v[1]), hi = i8_pack_bf2(v[2], v[3]);
+  if (n + 4 <= n_end) {
+    *reinterpret_cast<u32x2_any*>(row + n) = u32x2_any{lo, hi};
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < n_end) row[n + e] = static_cast<unsigned short>((e < 2 ? lo : hi) >> (16 * (e & 1)));
 }
 
 // The results of a wave's kT token blocks (16 tokens each, rows m0 ..) x 64 channels (n0 ..).  acc_of(j, t) is the lane's accumulator quad of channel
@@ -227,93 +250,70 @@ __device__ __forceinline__ void i8_store(const GemmI8Args& g, long m, int n, con
 template <bool kOut32, int kForm, int kT, bool kStream, typename AccOf, typename AsOf, typename BsOf, typename BiasOf>
 __device__ __forceinline__ void i8_store_tile(const GemmI8Args& g, long m0, int n0, int li, int lg, AccOf acc_of, AsOf as_of, BsOf bs_of, BiasOf bias_of) {
   constexpr int kN = kOut32 ? 4 : 8, kGap = kOut32 ? 16 : 32;
-  if constexpr (kForm == kI8Any) {
+  const bool low = li < 8;
+  constexpr int kMost = kForm >= kI8Residual && !kOut32 ? (kT == 8 ? 1 : 2) : 4, kGroup = kT < kMost ? kT : kMost;      // token blocks whose residual rows are in flight together
 #pragma unroll
-    for (int b = 0; b < 16 / kN; ++b) {
-      const int nl = kOut32 ? 16 * b + 4 * lg : 32 * b + 8 * lg;
-      if (n0 + nl >= g.N) continue;
-      float bs[kN], bias[kN];
+  for (int b = 0; b < 8 / kN; ++b) {             // pairs of pieces
+    const int nl = kOut32 ? 32 * b + 4 * lg : 8 * lg;
+    if (n0 + nl >= g.N) continue;
+    float bs[2][kN], bias[2][kN];
 #pragma unroll
-      for (int e = 0; e < kN; ++e) { bs[e] = bs_of(nl + e); bias[e] = bias_of(nl + e); }
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        const long m = m0 + 16 * t + li;
-        if (m >= g.M) continue;
-        int z[kN];
+      for (int e = 0; e < kN; ++e) { bs[h][e] = bs_of(nl + h * kGap + e); bias[h][e] = bias_of(nl + h * kGap + e); }
+    const int n = n0 + nl + (low ? 0 : kGap);    // of the two pieces that this lane stores, in rows li & 7 and 8 + (li & 7)
+    const bool in = n < g.N;
 #pragma unroll
-        for (int e = 0; e < kN; ++e) z[e] = kOut32 ? acc_of(b, t)[e & 3] : acc_of(2 * b + (e >> 2), t)[e & 3];
-        i8_store<kOut32, kN>(g, m, n0 + nl, z, as_of(t), bs, bias);
-      }
-    }
-  } else {
-    const bool low = li < 8;
-    constexpr int kGroup = kForm == kI8Residual && !kOut32 ? 2 : 4;      // token blocks whose residual rows are in flight together
-#pragma unroll
-    for (int b = 0; b < 8 / kN; ++b) {           // pairs of pieces
-      const int nl = kOut32 ? 32 * b + 4 * lg : 8 * lg;
-      if (n0 + nl >= g.N) continue;              // (N is a multiple of 8: the second pieces are checked on their own)
-      float bs[2][kN], bias[2][kN];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < kN; ++e) { bs[h][e] = bs_of(nl + h * kGap + e); bias[h][e] = bias_of(nl + h * kGap + e); }
-      const int n = n0 + nl + (low ? 0 : kGap);  // of the two pieces that this lane stores, in rows li & 7 and 8 + (li & 7)
-      const bool in = n < g.N;
-#pragma unroll
-      for (int t0 = 0; t0 < kT; t0 += kGroup) {
-        f32x4 ahead[kForm == kI8Residual ? kGroup : 1][kOut32 ? 2 : 4];
-        if constexpr (kForm == kI8Residual) {
-#pragma unroll
-          for (int t = 0; t < kGroup; ++t) {
-#pragma unroll
-            for (int q = 0; q < (kOut32 ? 2 : 4); ++q) {      // fp32: the two pieces as they are stored; bf16: four quads as they are computed
-              const long m = min(m0 + 16 * (t0 + t) + (kOut32 ? 8 * q + (li & 7) : li), static_cast<long>(g.M) - 1);
-              const int c = kOut32 ? n : n0 + nl + (q >> 1) * kGap + 4 * (q & 1);
-              ahead[t][q] = g.residual && c < g.N ? *reinterpret_cast<const f32x4*>(i8_residual(g, m, c)) : f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-          }
-        }
+    for (int t0 = 0; t0 < kT; t0 += kGroup) {
+      f32x4 ahead[kForm >= kI8Residual ? kGroup : 1][kOut32 ? 2 : 4];
+      if constexpr (kForm >= kI8Residual) {
 #pragma unroll
         for (int t = 0; t < kGroup; ++t) {
-          const float as = as_of(t0 + t);
-          unsigned w[2][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float z[kN];
-#pragma unroll
-            for (int e = 0; e < kN; ++e) {
-              const int a = kOut32 ? acc_of(2 * b + h, t0 + t)[e & 3] : acc_of(2 * h + (e >> 2), t0 + t)[e & 3];
-              z[e] = static_cast<float>(a) * as * bs[h][e] + bias[h][e];
-              if (kForm == kI8Gelu) z[e] = i8_gelu(z[e]);
-              if (kForm == kI8Residual && !kOut32) z[e] += ahead[t][(2 * h + (e >> 2)) & (kOut32 ? 1 : 3)][e & 3];
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) w[h][q] = kOut32 ? __float_as_uint(z[q]) : i8_pack_bf2(z[(2 * q) % kN], z[(2 * q + 1) % kN]);
+          for (int q = 0; q < (kOut32 ? 2 : 4); ++q) {        // fp32: the two pieces as they are stored; bf16: four quads as they are computed
+            const long m = min(m0 + 16 * (t0 + t) + (kOut32 ? 8 * q + (li & 7) : li), static_cast<long>(g.M) - 1);
+            const int c = kOut32 ? n : n0 + nl + (q >> 1) * kGap + 4 * (q & 1);
+            ahead[t][q] = g.residual && c < g.N ? i8_residual4(g, m, c) : f32x4{0.f, 0.f, 0.f, 0.f};
           }
-          u32x4 s[2];
+        }
+      }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const unsigned give = low ? w[1][q] : w[0][q];
-            const unsigned got = __builtin_amdgcn_update_dpp(give, give, 0x128, 0xf, 0xf, false);      // row_ror:8: lane li ^ 8
-            s[0][q] = low ? w[0][q] : got;
-            s[1][q] = low ? got : w[1][q];
+      for (int t = 0; t < kGroup; ++t) {
+        const float as = as_of(t0 + t);
+        unsigned w[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float z[kN];
+#pragma unroll
+          for (int e = 0; e < kN; ++e) {
+            const int a = kOut32 ? acc_of(2 * b + h, t0 + t)[e & 3] : acc_of(2 * h + (e >> 2), t0 + t)[e & 3];
+            z[e] = static_cast<float>(a) * as * bs[h][e] + bias[h][e];
+            if (kForm == kI8Gelu) z[e] = i8_gelu(z[e]);
+            if (kForm == kI8Any) z[e] = g.act == 1 ? i8_gelu(z[e]) : (g.act == 2 ? fmaxf(z[e], 0.f) : z[e]);
+            if (kForm >= kI8Residual && !kOut32) z[e] += ahead[t][(2 * h + (e >> 2)) & (kOut32 ? 1 : 3)][e & 3];
           }
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const long m = m0 + 16 * (t0 + t) + 8 * r + (li & 7);
-            if (!in || m >= g.M) continue;
-            if constexpr (kOut32) {
-              f32x4 v = __builtin_bit_cast(f32x4, s[r]);
-              if (kForm == kI8Residual) v += ahead[t][r];
-              f32x4* c = reinterpret_cast<f32x4*>(static_cast<float*>(g.C) + m * g.ldc + n);
-              if (kStream) __builtin_nontemporal_store(v, c);
-              else *c = v;
-              if (kForm == kI8Residual && g.aux) *reinterpret_cast<uint2*>(g.aux + m * g.ld_aux + n) = make_uint2(i8_pack_bf2(v[0], v[1]), i8_pack_bf2(v[2], v[3]));
-            } else {
-              u32x4* c = reinterpret_cast<u32x4*>(static_cast<unsigned short*>(g.C) + m * g.ldc + n);
-              if (kStream) __builtin_nontemporal_store(s[r], c);
-              else *c = s[r];
-            }
+          for (int q = 0; q < 4; ++q) w[h][q] = kOut32 ? __float_as_uint(z[q]) : i8_pack_bf2(z[(2 * q) % kN], z[(2 * q + 1) % kN]);
+        }
+        u32x4 s[2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const unsigned give = low ? w[1][q] : w[0][q];
+          const unsigned got = __builtin_amdgcn_update_dpp(give, give, 0x128, 0xf, 0xf, false);        // row_ror:8: lane li ^ 8
+          s[0][q] = low ? w[0][q] : got;
+          s[1][q] = low ? got : w[1][q];
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const long m = m0 + 16 * (t0 + t) + 8 * r + (li & 7);
+          if (!in || m >= g.M) continue;
+          if constexpr (kOut32) {
+            f32x4 v = __builtin_bit_cast(f32x4, s[r]);
+            if (kForm >= kI8Residual) v += ahead[t][r];
+            i8_put_f32<kStream>(static_cast<float*>(g.C) + m * g.ldc, n, g.N, v, g.stream);
+            if (kForm >= kI8Residual && g.aux) i8_put_copy(g.aux + m * g.ld_aux, n, g.N, v);
+          } else {
+            i8_put_bf16<kStream>(static_cast<unsigned short*>(g.C) + m * g.ldc, n, g.N, s[r], g.stream);
           }
         }
       }
@@ -321,90 +321,125 @@ __device__ __forceinline__ void i8_store_tile(const GemmI8Args& g, long m0, int 
   }
 }
 
-// ---- 128 x 128 tile, four waves (2 x 2, 64 x 64 each), K in steps of 128 bytes, two LDS stages filled by LDS-DMA
-constexpr int kI8Tile = 128 * 128;               // one operand's stage: 128 rows x 128 bytes
-constexpr int kI8Lds = 4 * kI8Tile;
+// ---- kTile x kTile tiles, K in steps of 128 bytes through a ring of kStages LDS stages filled by LDS-DMA
+//
+// 128: 2 x 2 waves of 64 tokens x 64 channels.  64: four pairs of waves of 16 tokens x 64 channels, half of every step each, which join at the end
+// (1000 x 1000 x 4800 in bf16 15.6 us with one wave each, 13.3 with two).  kStages - 1 steps are on their way while one is multiplied: a
+// call whose tiles leave CUs idle is bound by the time of a step's round trip, and the ring divides that by its depth.
+// One barrier a step: behind it step s has landed for every wave, and every wave has read what step s + kStages - 1 is fetched over.
 __device__ __attribute__((aligned(16))) unsigned g_i8_zero[4];
 // position p of LDS row r holds the row's 16-byte piece p ^ f(r); f makes the 16 rows of a fragment read fall on all eight positions twice
 __device__ __forceinline__ int i8_swz_natural(int row) { return (row >> 1) & 7; }
 __device__ __forceinline__ int i8_swz_bf16(int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); }
 
-template <bool kOut32, int kForm>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(GemmI8Args g, int tiles_m, int tiles_n) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [2 stages][token tile | weight tile]
+// LDS-DMA as inline asm without results: through the builtin the compiler takes every later LDS read to depend on it and waits for all
+// fetches in front of it.  The waits are the explicit ones of the schedule.
+__device__ __forceinline__ unsigned i8_lds_addr(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
+}
+__device__ __forceinline__ void i8_dma16(const void* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void i8_dma4(const void* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(src), "s"(lds) : "memory");
+}
+
+constexpr int i8_tile_lds(int tile, int stages) { return stages * 2 * tile * 128; }
+template <bool kOut32, int kForm, int kTile, int kStages>
+__global__ __launch_bounds__(kTile == 64 ? 512 : 256) void gemm_i8_kernel(GemmI8Args g, int tiles_m, int tiles_n) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // [stage][token tile | weight tile]
+  constexpr int kOp = kTile * 128, kTok = kTile == 128 ? 4 : 1, kDma = kTile == 128 ? 4 : 1;      // bytes of an operand's stage; a wave's token blocks; its fetches of an operand
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = kTile == 128 ? wave >> 1 : wave & 3, wn = kTile == 128 ? wave & 1 : 0;
+  constexpr int kKs = kTile == 128 ? 2 : 1;      // of a step's two halves, those that a wave multiplies
+  const int ks0 = kTile == 128 ? 0 : wave >> 2;
   // blocks b and b + 8 share an XCD and its L2: every XCD gets a contiguous range of tiles, the tiles of a token panel side by side
   const int nwg = tiles_m * tiles_n, bid = blockIdx.x;
   const int q8 = nwg >> 3, r8 = nwg & 7, xcd = bid & 7;
   const int logical = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (bid >> 3);
-  const int m0 = (logical / tiles_n) * 128, n0 = (logical % tiles_n) * 128;
+  const int m0 = (logical / tiles_n) * kTile, n0 = (logical % tiles_n) * kTile;
   const int steps = (g.K + 127) >> 7;
 
-  // DMA instruction i of this wave fills rows 8 (4 wave + i) .. + 7 of a tile, 16 bytes per lane; rows past the matrix are the last one's
-  const signed char *pa[4], *pb[4];
-  int ka[4], kb[4];
+  // fetch i of this wave fills rows 8 (kDma wave + i) .. + 7 of a tile, 16 bytes per lane; rows past the matrix are the last one's
+  const signed char *pa[kDma], *pb[kDma];
+  int ka[kDma], kb[kDma];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = 8 * (4 * wave + i) + (lane >> 3);
+  for (int i = 0; i < kDma; ++i) {
+    const int row = 8 * (kDma * wave + i) + (lane >> 3);
     ka[i] = ((lane & 7) ^ i8_swz_natural(row)) * 16;
     kb[i] = ((lane & 7) ^ (kOut32 ? i8_swz_natural(row) : i8_swz_bf16(row))) * 16;
     const int ar = min(m0 + row, g.M - 1), br = min(n0 + row, g.N - 1);
     pa[i] = g.A + static_cast<long>(ar) * g.lda + ka[i];
     pb[i] = g.B + static_cast<long>(br) * g.ldb + kb[i];
   }
-  auto dma = [&](int step) {
-    unsigned char* st = smem + (step & 1) * 2 * kI8Tile;
+  const unsigned lds0 = i8_lds_addr(smem);
+  auto dma = [&](int step, int stage) {          // steps past the end fetch zeros into stages that nobody reads, so that the counts stay exact
+    const unsigned st = lds0 + stage * 2 * kOp + kDma * wave * 1024;
     const int k0 = step * 128;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {                // pieces past K are zeros on both sides
-      const void* sa = k0 + ka[i] < g.K ? static_cast<const void*>(pa[i] + k0) : static_cast<const void*>(g_i8_zero);
-      const void* sb = k0 + kb[i] < g.K ? static_cast<const void*>(pb[i] + k0) : static_cast<const void*>(g_i8_zero);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)sa, (__attribute__((address_space(3))) void*)(st + (4 * wave + i) * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)sb, (__attribute__((address_space(3))) void*)(st + kI8Tile + (4 * wave + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < kDma; ++i) {             // pieces past K are zeros on both sides
+      i8_dma16(k0 + ka[i] < g.K ? static_cast<const void*>(pa[i] + k0) : static_cast<const void*>(g_i8_zero), st + i * 1024);
+      i8_dma16(k0 + kb[i] < g.K ? static_cast<const void*>(pb[i] + k0) : static_cast<const void*>(g_i8_zero), st + kOp + i * 1024);
     }
   };
   const int li = lane & 15, lg = lane >> 4, sw = (li >> 1) & 7;
-  int xr[4], wr[4];
+  int xr[kTok], wr[4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    xr[t] = (wm * 64 + 16 * t + li) * 128;
-    wr[t] = kI8Tile + (wn * 64 + (kOut32 ? 16 * t + li : w_row_bf16(t, li))) * 128;
-  }
-  i32x4 acc[4][4];                               // [weight block][token block]
+  for (int t = 0; t < kTok; ++t) xr[t] = (wm * 16 * kTok + 16 * t + li) * 128;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) wr[t] = kOp + (wn * 64 + (kOut32 ? 16 * t + li : w_row_bf16(t, li))) * 128;
+  i32x4 acc[4][kTok];                            // [weight block][token block]
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-  dma(0);
-  __syncthreads();
+    for (int j = 0; j < kTok; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) dma(s, s);
+  int stage = 0;
   for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) dma(s + 1);
-    const unsigned char* st = smem + (s & 1) * 2 * kI8Tile;
-    i32x4 xf[2][4], wf[2][4];
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"((kStages - 2) * 2 * kDma) : "memory");
+    asm volatile("s_barrier" ::: "memory");
+    const int last = stage == 0 ? kStages - 1 : stage - 1;
+    dma(s + kStages - 1, last);
+    const unsigned char* st = smem + stage * 2 * kOp;
+    i32x4 xf[kKs][kTok], wf[kKs][4];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int ks = 0; ks < kKs; ++ks) {
+      const int c = ((4 * (ks0 + ks) + lg) ^ sw) * 16;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int c = ((4 * ks + lg) ^ sw) * 16;
-        xf[ks][t] = *reinterpret_cast<const i32x4*>(st + xr[t] + c);
-        wf[ks][t] = *reinterpret_cast<const i32x4*>(st + wr[t] + c);
-      }
+      for (int t = 0; t < kTok; ++t) xf[ks][t] = *reinterpret_cast<const i32x4*>(st + xr[t] + c);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+      for (int t = 0; t < 4; ++t) wf[ks][t] = *reinterpret_cast<const i32x4*>(st + wr[t] + c);
+    }
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[ks][i], xf[ks][j], acc[i][j], 0, 0, 0);
-    __syncthreads();
+        for (int j = 0; j < kTok; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[ks][i], xf[ks][j], acc[i][j], 0, 0, 0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // (the reads are done in front of the next barrier)
+    stage = stage == kStages - 1 ? 0 : stage + 1;
   }
-  float as[4];
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // no fetch outlives its workgroup's LDS
+  if constexpr (kTile == 64) {                   // the two waves of a block join, one integer sum
+    __syncthreads();
+    i32x4* const part = reinterpret_cast<i32x4*>(smem) + wm * 256 + lane;
+    if (wave >= 4) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) as[j] = g.a_scale[min(m0 + wm * 64 + 16 * j + li, g.M - 1)];
+      for (int i = 0; i < 4; ++i) part[64 * i] = acc[i][0];
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i][0] += part[64 * i];
+  }
+  float as[kTok];
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) as[j] = g.a_scale[min(m0 + wm * 16 * kTok + 16 * j + li, g.M - 1)];
   const int nw = n0 + wn * 64;
-  i8_store_tile<kOut32, kForm, 4, false>(g, m0 + wm * 64, nw, li, lg, [&](int i, int j) { return acc[i][j]; }, [&](int j) { return as[j]; },
-                                         [&](int c) { return g.b_scale[min(nw + c, g.N - 1)]; }, [&](int c) { return g.bias ? g.bias[min(nw + c, g.N - 1)] : 0.f; });
+  i8_store_tile<kOut32, kForm, kTok, false>(g, m0 + wm * 16 * kTok, nw, li, lg, [&](int i, int j) { return acc[i][j]; }, [&](int j) { return as[j]; },
+                                            [&](int c) { return g.b_scale[min(nw + c, g.N - 1)]; }, [&](int c) { return g.bias ? g.bias[min(nw + c, g.N - 1)] : 0.f; });
 }
 
 // ---- few tokens: 16 kMT tokens x 16 channels per workgroup, K dealt in steps of 64 bytes over its eight waves, which join through LDS
@@ -525,7 +560,21 @@ __global__ __launch_bounds__(64 * kI8SkinnyWaves) void gemm_i8_skinny_kernel(Gem
 #pragma unroll
     for (int w = 0; w < kW; ++w) z[j] += part[w][er][c];
   }
-  i8_store<kOut32, 4>(g, em, en, z, kX == kXInt8 ? eas : srow[er & 15], ebs, ebias);
+  const float as = kX == kXInt8 ? eas : srow[er & 15];
+  f32x4 y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    y[j] = static_cast<float>(z[j]) * as * ebs[j] + ebias[j];
+    if (g.act == 1) y[j] = i8_gelu(y[j]);
+    else if (g.act == 2) y[j] = fmaxf(y[j], 0.f);
+  }
+  if (g.residual) y += i8_residual4(g, em, en);
+  if (kOut32) {
+    i8_put_f32<false>(static_cast<float*>(g.C) + em * g.ldc, en, g.N, y, false);
+    if (g.aux) i8_put_copy(g.aux + em * g.ld_aux, en, g.N, y);
+  } else {
+    i8_put_copy(static_cast<unsigned short*>(g.C) + em * g.ldc, en, g.N, y);
+  }
 }
 
 // ---- 256 x 256 tile, eight waves (2 x 4, 128 tokens x 64 channels each), K in steps of 128 bytes, one persistent workgroup per CU
@@ -550,19 +599,8 @@ constexpr int kI8Half = 128 * 128;
 constexpr int kI8Buf = 4 * kI8Half;              // A_0 | A_1 | B_0 | B_1
 constexpr int kI8Scales = 3 * 256 * 4;           // a_scale | b_scale | bias of a tile
 constexpr int kI8BigLds = 2 * kI8Buf + 2 * kI8Scales;
-__device__ __forceinline__ unsigned i8_lds_addr(const void* p) {
-  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
-}
-// LDS-DMA as inline asm without results: through the builtin the compiler takes every later LDS read to depend on it and waits for all
-// fetches in front of it.  The waits are the explicit ones of the schedule.
-__device__ __forceinline__ void i8_dma16(const void* src, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(src), "s"(lds) : "memory");
-}
-__device__ __forceinline__ void i8_dma4(const void* src, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(src), "s"(lds) : "memory");
-}
 
-template <bool kOut32, int kForm>
+template <bool kOut32, int kForm, bool kTail>
 __global__ __launch_bounds__(512) void gemm_i8_256_kernel(GemmI8Args g, int tiles_m, int tiles_n, int group_n) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -610,7 +648,7 @@ __global__ __launch_bounds__(512) void gemm_i8_256_kernel(GemmI8Args g, int tile
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const void* src = p[j] + static_cast<long>(s) * 128;
-      if (kForm == kI8Any) src = s * 128 + kc[j] < g.K ? src : static_cast<const void*>(g_i8_zero);      // (the other forms: K a multiple of 128)
+      if (kTail) src = s * 128 + kc[j] < g.K ? src : static_cast<const void*>(g_i8_zero);      // (else K is a multiple of 128)
       i8_dma16(src, lds0 + buf * kI8Buf + half * kI8Half + (2 * wave + j) * 1024);
     }
   };
@@ -739,7 +777,8 @@ __global__ __launch_bounds__(512) void gemm_i8_256_kernel(GemmI8Args g, int tile
 using namespace adt;
 
 namespace adt {
-// Lanes per row: the fewest that hold the row in at most three pieces each, so that no lane idles (768 columns: 32 lanes, three pieces)
+// Lanes per row: the fewest that hold the row in at most three pieces each, so that no lane idles (768 columns: 32 lanes, three pieces); a whole
+// workgroup past 2048 columns (us with 64 / 256 lanes, fp32: 4096 x 4096 17.2 / 14.0, 2048 x 8192 23.1 / 13.9, 1 x 3400 4.1 / 2.6)
 template <bool kF32, int kLanes, int kP>
 static void launch_quant_as(const QuantArgs& a, bool vec, hipStream_t st) {
   constexpr int kRows = 256 / kLanes;
@@ -756,9 +795,9 @@ static void launch_quant(const QuantArgs& a, bool vec, hipStream_t st) {
   else if (pieces <= 128) launch_quant_as<kF32, 64, 2>(a, vec, st);
   else if (pieces <= 192) launch_quant_as<kF32, 64, 3>(a, vec, st);
   else if (pieces <= 256) launch_quant_as<kF32, 64, 4>(a, vec, st);
-  else if (pieces <= 384) launch_quant_as<kF32, 64, 6>(a, vec, st);
-  else if (pieces <= 512) launch_quant_as<kF32, 64, 8>(a, vec, st);
-  else launch_quant_as<kF32, 64, 0>(a, vec, st);
+  else if (pieces <= 512) launch_quant_as<kF32, 256, 2>(a, vec, st);
+  else if (pieces <= 1024) launch_quant_as<kF32, 256, 4>(a, vec, st);
+  else launch_quant_as<kF32, 256, 0>(a, vec, st);
 }
 }  // namespace adt
 
@@ -800,9 +839,8 @@ static GemmI8Args gemm_i8_args(int64_t M, int64_t N, int64_t Kp, const void* B, 
   g.B = static_cast<const signed char*>(B); g.ldb = ldb; g.b_scale = b_scale;
   g.C = C; g.ldc = ldc; g.bias = ep->bias; g.residual = static_cast<const float*>(ep->residual); g.ld_res = ep->ld_res; g.res_row_mod = ep->res_row_mod;
   g.aux = static_cast<unsigned short*>(ep->aux_bf16_out); g.ld_aux = ep->ld_aux;
-  g.M = static_cast<int>(M); g.N = static_cast<int>(N); g.K = static_cast<int>(Kp); g.act = ep->act;
-  auto ok = [](const void* p, int64_t ld, int elem) { return !p || (aligned16(p) && (ld * elem) % 16 == 0); };
-  g.vec = (N % 8) == 0 && ok(C, ldc, ep->out_fp32 ? 4 : 2) && ok(g.bias, 4, 4) && ok(b_scale, 4, 4) && ok(g.residual, g.ld_res, 4) && ok(g.aux, g.ld_aux, 2);
+  g.M = static_cast<int>(M); g.N = static_cast<int>(N); g.K = static_cast<int>(Kp); g.act = ep->act; 
+  g.stream = (reinterpret_cast<uintptr_t>(C) & 127) == 0 && (ldc * (ep->out_fp32 ? 4 : 2)) % 128 == 0;
   return g;
 }
 template <bool kOut32, int kMT, int kX>
@@ -812,30 +850,43 @@ static int launch_i8_skinny(const GemmI8Args& g, const LinearX& lx, hipStream_t 
   ADT_HIP_TRY(hipGetLastError());
   return ADT_OK;
 }
+template <bool kOut32, int kTile, int kStages>
+static int launch_i8_tile(const GemmI8Args& g, int form, int64_t tm, int64_t tn, hipStream_t st) {
+  typedef void (*Fn)(GemmI8Args, int, int);
+  static const Fn fns[4] = {gemm_i8_kernel<kOut32, 0, kTile, kStages>, gemm_i8_kernel<kOut32, 1, kTile, kStages>, gemm_i8_kernel<kOut32, 2, kTile, kStages>,
+                            gemm_i8_kernel<kOut32, 3, kTile, kStages>};
+  if (tm * tn > (1LL << 31) - 1) return set_error(ADT_ESHAPE, "adt_gemm_i8: too many tiles");
+  constexpr int kLds = i8_tile_lds(kTile, kStages);
+  if (kLds > 65536) ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(fns[form]), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+  hipLaunchKernelGGL(fns[form], dim3(static_cast<unsigned>(tm * tn)), dim3(kTile == 64 ? 512 : 256), kLds, st, g, static_cast<int>(tm), static_cast<int>(tn));
+  ADT_HIP_TRY(hipGetLastError());
+  return ADT_OK;
+}
 template <bool kOut32>
 static int launch_i8(const GemmI8Args& g, hipStream_t st) {
-  typedef void (*Fn)(GemmI8Args, int, int);
   typedef void (*BigFn)(GemmI8Args, int, int, int);
-  static const Fn fns[4] = {gemm_i8_kernel<kOut32, 0>, gemm_i8_kernel<kOut32, 1>, gemm_i8_kernel<kOut32, 2>, gemm_i8_kernel<kOut32, 3>};
-  static const BigFn big[4] = {gemm_i8_256_kernel<kOut32, 0>, gemm_i8_256_kernel<kOut32, 1>, gemm_i8_256_kernel<kOut32, 2>, gemm_i8_256_kernel<kOut32, 3>};
+  static const BigFn big[2][4] = {{gemm_i8_256_kernel<kOut32, 0, false>, gemm_i8_256_kernel<kOut32, 1, false>, gemm_i8_256_kernel<kOut32, 2, false>, gemm_i8_256_kernel<kOut32, 3, false>},
+                                  {gemm_i8_256_kernel<kOut32, 0, true>, gemm_i8_256_kernel<kOut32, 1, true>, gemm_i8_256_kernel<kOut32, 2, true>, gemm_i8_256_kernel<kOut32, 3, true>}};
   int n_cu = 0;
   if (int rc = device_cu_count(&n_cu)) return rc;
   const bool extra = g.residual || g.aux;
-  int form = kI8Any;
-  if (g.vec) form = g.act == 0 ? (extra ? kI8Residual : kI8Plain) : (g.act == 1 && !extra ? kI8Gelu : kI8Any);
-  const int64_t tm = (g.M + 127) / 128, tn = (g.N + 127) / 128, bm = (g.M + 255) / 256, bn = (g.N + 255) / 256;
-  // Few tokens: while its workgroups of 64 tokens x 16 channels are at most two per CU, the kernel that asks for everything at once wins
-  // (768 deep, us here / with 128 x 128 tiles: 64 x 1400 4.3 / 7.6, 256 x 768 4.3 / 7.7, 256 x 2304 8.3 / 7.9, 512 x 768 6.3 / 7.7, 1024 x 768 8.6 / 7.8).
-  if (static_cast<int64_t>((g.M + 63) / 64) * ((g.N + 15) / 16) <= 2 * n_cu && (g.M + 15) / 16 <= 65535) {
+  const int form = g.act == 0 ? (extra ? kI8Residual : kI8Plain) : (g.act == 1 && !extra ? kI8Gelu : kI8Any);
+  const int64_t tm = (g.M + 127) / 128, tn = (g.N + 127) / 128, bm = (g.M + 255) / 256, bn = (g.N + 255) / 256, sm = (g.M + 63) / 64, sn = (g.N + 63) / 64;
+  // Few tokens: the kernel that asks for everything at once, while its workgroups of up to 64 tokens x 16 channels are one a CU, or two where they hold
+  // no more than 32 tokens; then 64 x 64 tiles while they are two a CU at most (us with 16 channels / 64 x 64 / 128 x 128 tiles: 200 x 1000 x 1000
+  // 4.0 / 5.0 / 9.2, 16 x 8000 x 768 3.7 / 4.7 / 7.5, 32 x 16000 x 768 7.3 / 4.8 / 7.7, 128 x 2304 x 768 6.2 / 4.7 / 8.0, 1024 x 768 x 768 8.8 / 4.9 / 8.0,
+  // 256 x 4096 x 4096 40 / 13.3 / 25.6; three tiles a CU, 1282 x 2263 x 137, 14.2 / 8.6 / 7.6).
+  if (sm * ((g.N + 15) / 16) <= (g.M <= 32 ? 2 : 1) * n_cu) {
     if (g.M <= 16) return launch_i8_skinny<kOut32, 1, kXInt8>(g, LinearX{}, st);
     if (g.M <= 32) return launch_i8_skinny<kOut32, 2, kXInt8>(g, LinearX{}, st);
     return launch_i8_skinny<kOut32, 4, kXInt8>(g, LinearX{}, st);
   }
+  if (sm * sn <= 2 * n_cu) return launch_i8_tile<kOut32, 64, 4>(g, form, sm, sn, st);
   // 256 x 256 tiles run one per CU and twice as efficiently, but in whole rounds: a round of them costs 1.6 of 128 x 128 ones at two per CU (us with
   // 256 / 128: 4096 x 2304 x 768 16.4 / 18.9, 7747 x 768 x 768 14.6 / 11.2, 8192 x 2304 x 768 29.4 / 29.3, 16384 x 2304 x 768 43.6 / 53.1,
   // 63104 x 2304 x 768 140 / 240, 2048 x 4096 x 4096 43.8 / 45.1, 4096^3 55.2 / 85.3).
   if (8 * ((bm * bn + n_cu - 1) / n_cu) <= 5 * ((tm * tn + 2 * n_cu - 1) / (2 * n_cu))) {
-    const BigFn fn = big[(g.K & 127) ? kI8Any : form];
+    const BigFn fn = big[(g.K & 127) != 0][form];
     ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, kI8BigLds));
     const int64_t wgs = bm * bn < n_cu ? bm * bn : n_cu;
     // tile columns walked together: as many as 2 MB of weights (half an XCD's L2) are, three at least; the token panels are then read once
@@ -843,8 +894,7 @@ static int launch_i8(const GemmI8Args& g, hipStream_t st) {
     const int group_n = static_cast<int>(std::max<int64_t>(3, std::min<int64_t>(bn, (2 << 20) / (256LL * g.K))));
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(wgs)), dim3(512), kI8BigLds, st, g, static_cast<int>(bm), static_cast<int>(bn), group_n);
   } else {
-    if (tm * tn > (1LL << 31) - 1) return set_error(ADT_ESHAPE, "adt_gemm_i8: too many tiles");
-    hipLaunchKernelGGL(fns[form], dim3(static_cast<unsigned>(tm * tn)), dim3(256), kI8Lds, st, g, static_cast<int>(tm), static_cast<int>(tn));
+    return launch_i8_tile<kOut32, 128, 2>(g, form, tm, tn, st);
   }
   ADT_HIP_TRY(hipGetLastError());
   return ADT_OK;

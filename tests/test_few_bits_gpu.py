@@ -27,7 +27,7 @@ def quant_ref(x):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("m,k", [(1, 1), (3, 7), (5, 16), (64, 768), (7, 1001), (130, 520), (2, 5000), (33, 64), (9, 8192)])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 7), (5, 16), (64, 768), (7, 1001), (130, 520), (2, 5000), (33, 64), (9, 8192), (3, 2049), (70, 4096), (2, 4099), (5, 20000)])
 def test_quant_rows_codes_are_the_nearest_integers(dtype, m, k):
     x = (torch.randn(m, k + 5, generator=gen(m * 1000 + k)) * torch.exp(torch.randn(m, 1, generator=gen(k)))).to(dtype).cuda()[:, 2:2 + k]
     q, s = K.quant_rows_i8(x)
@@ -136,6 +136,37 @@ def test_gemm_i8_views_periodic_residual_and_bf16_copy(m):
         assert (w32[:, :lo] == 7).all() and (w32[:, lo + w:] == 7).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(20, 1001, 80), (40, 301, 2000), (300, 1003, 400), (1282, 2263, 144), (4400, 2301, 640), (4400, 2304, 640), (1, 1, 16)])
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_gemm_i8_odd_widths_activation_residual_and_what_lies_around(m, n, k, out):
+    """Every tile size at widths that no 16-byte piece divides, rows that begin anywhere, and the whole epilogue at once."""
+    g = gen(m + n + k)
+    a, b = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((m, k), (n, k)))
+    sa, sb = (0.5 + torch.rand(m, generator=g)).cuda() / 127, (0.5 + torch.rand(n, generator=g)).cuda() / (127 * math.sqrt(k) / 3)
+    bias, res = torch.randn(n, generator=g).cuda(), torch.randn(m, n + 3, generator=g).cuda()[:, 2:2 + n]
+    for lo, width, r, act in ((0, n, res, 1), (3, n + 7, None, 2), (5, n + 6, res, 0)):
+        wide = torch.full((m, width + lo), 7.0, device="cuda", dtype=out)
+        copy = torch.full((m, width + lo), 7.0, device="cuda", dtype=BF16) if out == F32 else None
+        o = wide[:, lo:lo + n]
+        K.gemm_i8(a, sa, b, sb, out=o, bias=bias, residual=r, act=act, aux_bf16_out=None if copy is None else copy[:, lo:lo + n])
+        check_product(a, sa, b, sb, o, bias, r, act)
+        assert (wide[:, :lo] == 7).all() and (wide[:, lo + n:] == 7).all()
+        if copy is not None:
+            assert torch.equal(copy[:, lo:lo + n], o.to(BF16)) and (copy[:, :lo] == 7).all() and (copy[:, lo + n:] == 7).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(7, 40, 64), (300, 776, 768), (1300, 2264, 144), (5000, 2304, 768)])
+def test_gemm_i8_adds_to_the_residual_in_place(m, n, k):
+    g = gen(m * n)
+    a, b = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((m, k), (n, k)))
+    sa, sb = torch.rand(m, generator=g).cuda() / 100, torch.rand(n, generator=g).cuda() / 100
+    x = torch.randn(m, n, generator=g).cuda()
+    expected = K.gemm_i8(a, sa, b, sb, out_dtype=F32, residual=x)
+    check_product(a, sa, b, sb, expected, residual=x)
+    K.gemm_i8(a, sa, b, sb, out=x, residual=x)
+    assert torch.equal(x, expected)
+
+
 def test_gemm_i8_sums_stay_exact_at_the_longest_k():
     k = 131072
     a = torch.full((3, k), 127, dtype=torch.int8, device="cuda")
@@ -148,7 +179,7 @@ def test_gemm_i8_sums_stay_exact_at_the_longest_k():
 
 
 @pytest.mark.parametrize("m", [1, 16, 40, 64, 65, 900])
-@pytest.mark.parametrize("k", [50, 768])
+@pytest.mark.parametrize("k", [50, 768, 2300])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_linear_i8_is_quantise_then_multiply(m, k, dtype):
     g = gen(m * k)
