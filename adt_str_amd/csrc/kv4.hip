@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <algorithm>
 #include <cstdio>
 
 #include "adt_common.h"
@@ -329,33 +330,35 @@ __device__ __forceinline__ float kv_scale_of(unsigned par) { return __uint_as_fl
 __device__ __forceinline__ float kv_min_of(unsigned par) { return __uint_as_float(par & 0xffff0000u); }
 
 template <int D, int kW>
-__global__ __launch_bounds__(64 * kW, kW == 4 ? 3 : 1) void attn_kv4_kernel(KvAttnArgs a, int n_max) {      // n_max = min(16, rows)
+__global__ __launch_bounds__(64 * kW, kW < 8 ? 3 : 1) void attn_kv4_kernel(KvAttnArgs a, int n_max) {      // n_max = min(16, rows)
   using R = KvRec<D>;
   constexpr int kG = R::kG, kNB = D / 16, kPieces = D / 64;          // V pieces (16 bytes) per lane and tile
   constexpr int kPitch = D + 4;
-  static_assert(64 * kW >= 2 * D, "a thread per sixteen bytes of q");
+  constexpr int kQ = (2 * D + 64 * kW - 1) / (64 * kW);              // sixteen-byte pieces of q per thread
   extern __shared__ __attribute__((aligned(16))) float so[];         // [kW][n_max][kPitch] at the end; the rows of q at the start
   __shared__ float sm[kW][16], sl[kW][16], sc[kW][kG][16];
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, u = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int id = blockIdx.x;
-  const int span = id % a.spans; id /= a.spans;
+  const int slot = id % a.spans; id /= a.spans;
+  const int span = (slot + id) % a.spans;      // (blocks b and b + 8 share an XCD: the late spans, empty in short sequences, are spread over them)
   const int rb = id % a.row_blocks; id /= a.row_blocks;
   const int hk = id % a.Hk, b = id / a.Hk;
   // ---- everything the first tile needs is asked for at once: the length, this block's rows of q (sixteen bytes per thread, two-byte loads where
   // the rows are not aligned), the tile itself (the span's last one at most, whatever the length is)
   int klen = a.key_len ? a.key_len[b] : a.cap;
-  u32x4 qw = {0u, 0u, 0u, 0u};
-  if (tid < 2 * D) {
-    const int row = rb * 16 + tid / (D / 8), c = 8 * (tid % (D / 8));
-    if (row < a.rows) {
-      const unsigned short* p = a.q + (static_cast<long>(b) * a.q_len + row / a.group) * a.ldq + (hk * a.group + row % a.group) * D + c;
-      if (a.qvec) {
-        qw = *reinterpret_cast<const u32x4*>(p);
-      } else {
+  u32x4 qw[kQ];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) qw[j] = p[2 * j] | static_cast<unsigned>(p[2 * j + 1]) << 16;
-      }
+  for (int i = 0; i < kQ; ++i) {
+    qw[i] = u32x4{0u, 0u, 0u, 0u};
+    const int piece = tid + 64 * kW * i, row = rb * 16 + piece / (D / 8), c = 8 * (piece % (D / 8));
+    if (piece >= 2 * D || row >= a.rows) continue;
+    const unsigned short* p = a.q + (static_cast<long>(b) * a.q_len + row / a.group) * a.ldq + (hk * a.group + row % a.group) * D + c;
+    if (a.qvec) {
+      qw[i] = *reinterpret_cast<const u32x4*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qw[i][j] = p[2 * j] | static_cast<unsigned>(p[2 * j + 1]) << 16;
     }
   }
   const unsigned char* const base = a.cache + static_cast<long>(b * a.Hk + hk) * a.tiles * R::kBytes;
@@ -397,8 +400,12 @@ __global__ __launch_bounds__(64 * kW, kW == 4 ? 3 : 1) void attn_kv4_kernel(KvAt
 
   unsigned short* const ql = reinterpret_cast<unsigned short*>(so);  // [16][D + 8]
   constexpr int kQPitch = D + 8;
-  if (a.negate) qw ^= 0x80008000u;
-  if (tid < 2 * D) *reinterpret_cast<u32x4*>(ql + (tid / (D / 8)) * kQPitch + 8 * (tid % (D / 8))) = qw;
+#pragma unroll
+  for (int i = 0; i < kQ; ++i) {
+    const int piece = tid + 64 * kW * i;
+    if (a.negate) qw[i] ^= 0x80008000u;
+    if (piece < 2 * D) *reinterpret_cast<u32x4*>(ql + (piece / (D / 8)) * kQPitch + 8 * (piece % (D / 8))) = qw[i];
+  }
   __syncthreads();
   KvFrag qf[D / 32];
   float qs[kG];
@@ -558,14 +565,22 @@ __global__ __launch_bounds__(64 * kW, kW == 4 ? 3 : 1) void attn_kv4_kernel(KvAt
   }
 }
 
-// One row per workgroup, a thread per channel: lane s weighs span s (at most 64 of them), the spans' outputs are then independent loads.
+// One row per workgroup: lane s weighs span s (at most 64 of them); the spans' outputs are dealt to 512 / D threads a channel, all loads at once
+// (a thread a channel: 37 spans 4 us more).
 template <int D>
-__global__ __launch_bounds__(D) void attn_kv4_join_kernel(KvAttnArgs a) {
+__global__ __launch_bounds__(512) void attn_kv4_join_kernel(KvAttnArgs a) {
+  constexpr int kS = 512 / D, kEach = kKvMaxSpans / kS;              // spans s = part_of, part_of + kS, ..: all of a thread's are asked for at once
+  __shared__ float so[kS][D];
   const int orow = blockIdx.x % a.rows, bh = blockIdx.x / a.rows, hk = bh % a.Hk, b = bh / a.Hk;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, d = threadIdx.x % D, part_of = threadIdx.x / D;
   const float* part = a.part + (static_cast<long>(bh) * a.rows + orow) * a.spans * (D + 2);
-  float ms = kKvNegBig, ls = 0.f;
+  float ms = kKvNegBig, ls = 0.f, ov[kEach];
   if (lane < a.spans) { ms = part[lane * (D + 2) + D]; ls = part[lane * (D + 2) + D + 1]; }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int s = part_of + kS * i;
+    ov[i] = s < a.spans ? part[s * (D + 2) + d] : 0.f;
+  }
   float mm = ms;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
@@ -573,12 +588,20 @@ __global__ __launch_bounds__(D) void attn_kv4_join_kernel(KvAttnArgs a) {
   float lt = f * ls, ot = 0.f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o);
-#pragma unroll 8
-  for (int s = 0; s < a.spans; ++s) ot = fmaf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s)), part[s * (D + 2) + threadIdx.x], ot);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const float fs = __shfl(f, part_of + kS * i);
+    if (part_of + kS * i < a.spans) ot = fmaf(fs, ov[i], ot);
+  }
+  so[part_of][d] = ot;
+  __syncthreads();
+  if (part_of) return;
+#pragma unroll
+  for (int s = 1; s < kS; ++s) ot += so[s][d];
   const int oi = orow / a.group, oh = hk * a.group + orow % a.group;
   const bool any = lt > 0.f || lt != lt;
-  a.out[(static_cast<long>(b) * a.q_len + oi) * a.ldo + oh * D + threadIdx.x] = static_cast<unsigned short>(kv_f2bf(any ? ot / lt : 0.f));
-  if (threadIdx.x == 0 && a.lse) a.lse[(static_cast<long>(b) * (a.Hk * a.group) + oh) * a.q_len + oi] = any ? (mm + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+  a.out[(static_cast<long>(b) * a.q_len + oi) * a.ldo + oh * D + d] = static_cast<unsigned short>(kv_f2bf(any ? ot / lt : 0.f));
+  if (d == 0 && a.lse) a.lse[(static_cast<long>(b) * (a.Hk * a.group) + oh) * a.q_len + oi] = any ? (mm + log2f(lt)) * 0.6931471805599453f : -INFINITY;
 }
 
 }  // namespace adt
@@ -609,22 +632,38 @@ static int kv_rows_check(const char* who, int64_t B, int64_t H, int64_t D, const
   return set_error(ADT_EINVAL, msg);
 }
 struct KvPlan { int rows, row_blocks, tiles, spans, span_tiles, waves; };
-// A wave takes 0.7 us per tile when it has its SIMD to itself (420 instructions), a call 5 us around its tiles and 2 us more for the join of spans.  With
-// at most a workgroup per CU: eight waves each, and spans until there is one per CU or a wave has one tile (us with waves / spans: 6 heads x 986
-// positions 8/4 8.1, 8/1 9.4, 4/1 10.5; 64 x 32000 8/4 67.8, 8/1 207, 4/8 67.6; 120 x 3001, 64 channels, 8/2 13.1, 4/1 17.5).  With more: four waves,
-// three workgroups fit a CU, and spans only where less than half of that is in use (384 x 986 4/1 17.9, 4/2 17.7, 8/1 18.9; 1536 x 986 43.4, 49.6, 52.4).
+// How a call is cut.  A wave's tile costs 1 us when it has its SIMD to itself (420 instructions), a call 5 us around its tiles and 2 us more for the
+// join of spans.  A workgroup of eight waves fills half a CU or more, of four a third.  us with waves / spans, heads x positions:
+//   at most one workgroup a CU and three tiles a wave: eight waves, one span (16 x 582 8/1 5.3, 4/1 5.4, 4/6 7.5);
+//   one to four rows: four waves, and spans until the card is full, or of 32 tiles, as short sequences leave theirs empty and the late
+//   ones even that out (6 x 986 4/8 7.3, 8/4 8.3, 8/1 9.6; 64 x 32000 in four rows, ragged, 4/24 39, 4/12 53, 8/4 55; 174 x 21483 4/24 41, 4/4 59, 8/2 74);
+//   more rows, whose joins weigh more: eight waves, spans for one workgroup a CU, or of 64 tiles (60 x 2359 in 16 rows 8/4 13.6, 4/12 15.1; 108 x 4271
+//   in 8 rows 8/2 14.8, 4/6 15.8);
+//   more workgroups than CUs: four waves, spans of 32 tiles (1536 x 986 4/1 40, 4/2 50, 8/1 52; 384 x 500 4/1 10.2, 4/2 12.4), and two waves where a sequence
+//   is five tiles at most (1440 x 85 2/1 8.0, 4/1 10.6).
+// Sixteen workgroups a CU are the most that spans make: past that nothing is left to even out, and the workspace stays under 35 MB.
 static int kv_plan(const adt_attn_kv4_desc* d, KvPlan* p) {
   int n_cu = 256;
   (void)device_cu_count(&n_cu);
   p->rows = d->q_len * (d->heads / d->kv_heads);
   p->row_blocks = (p->rows + 15) / 16;
   p->tiles = (d->capacity + kKvTile - 1) / kKvTile;
-  const long wgs = static_cast<long>(d->batch) * d->kv_heads * p->row_blocks;
-  p->waves = wgs <= n_cu ? 8 : 4;
-  long want = wgs <= 0 ? 1 : (p->waves == 8 ? (n_cu + wgs - 1) / wgs : 5L * n_cu / (2 * wgs));
-  const long most = (p->tiles + p->waves - 1) / p->waves;
-  want = want > most ? most : want;
-  want = want < 1 ? 1 : (want > kKvMaxSpans ? kKvMaxSpans : want);
+  const int64_t wgs = static_cast<int64_t>(d->batch) * d->kv_heads * p->row_blocks;
+  int64_t want = 1;
+  if (wgs > n_cu) {
+    p->waves = wgs > 2 * n_cu && p->tiles <= 5 ? 2 : 4;
+    want = (p->tiles + 16) / 32;
+  } else if (p->tiles <= 26) {
+    p->waves = 8;
+  } else if (p->rows <= 4) {
+    p->waves = 4;
+    want = std::max<int64_t>(3 * n_cu / std::max<int64_t>(wgs, 1), (p->tiles + 16) / 32);
+  } else {
+    p->waves = 8;
+    want = std::max<int64_t>(n_cu / std::max<int64_t>(wgs, 1), (p->tiles + 32) / 64);
+  }
+  const int64_t most = std::min({static_cast<int64_t>((p->tiles + p->waves - 1) / p->waves), static_cast<int64_t>(kKvMaxSpans), 16 * n_cu / std::max<int64_t>(wgs, 1)});
+  want = std::max<int64_t>(1, std::min(want, most));
   p->span_tiles = static_cast<int>((p->tiles + want - 1) / want);
   p->spans = (p->tiles + p->span_tiles - 1) / p->span_tiles;
   return ADT_OK;
@@ -718,11 +757,14 @@ extern "C" int adt_attn_kv4(const adt_attn_kv4_desc* d, const void* q, const voi
   const int64_t wgs = static_cast<int64_t>(d->batch) * d->kv_heads * p.row_blocks * p.spans, joins = static_cast<int64_t>(d->batch) * d->kv_heads * p.rows;
   if (wgs > (1LL << 31) - 1 || joins > (1LL << 31) - 1) return set_error(ADT_ESHAPE, "adt_attn_kv4: too many workgroups");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const auto launch = d->head_dim == 128 ? (p.waves == 8 ? launch_attn_kv4<128, 8> : launch_attn_kv4<128, 4>) : (p.waves == 8 ? launch_attn_kv4<64, 8> : launch_attn_kv4<64, 4>);
+  typedef int (*Launch)(const KvAttnArgs&, unsigned, hipStream_t);
+  static const Launch launches[2][4] = {{launch_attn_kv4<64, 1>, launch_attn_kv4<64, 2>, launch_attn_kv4<64, 4>, launch_attn_kv4<64, 8>},
+                                        {launch_attn_kv4<128, 1>, launch_attn_kv4<128, 2>, launch_attn_kv4<128, 4>, launch_attn_kv4<128, 8>}};
+  const Launch launch = launches[d->head_dim == 128][p.waves == 8 ? 3 : p.waves / 2];
   if (int rc = launch(a, static_cast<unsigned>(wgs), st)) return rc;
   if (p.spans > 1) {
-    if (d->head_dim == 128) hipLaunchKernelGGL(attn_kv4_join_kernel<128>, dim3(static_cast<unsigned>(joins)), dim3(128), 0, st, a);
-    else hipLaunchKernelGGL(attn_kv4_join_kernel<64>, dim3(static_cast<unsigned>(joins)), dim3(64), 0, st, a);
+    if (d->head_dim == 128) hipLaunchKernelGGL(attn_kv4_join_kernel<128>, dim3(static_cast<unsigned>(joins)), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL(attn_kv4_join_kernel<64>, dim3(static_cast<unsigned>(joins)), dim3(512), 0, st, a);
     ADT_HIP_TRY(hipGetLastError());
   }
   return ADT_OK;

@@ -414,6 +414,23 @@ def test_attn_kv4_long_contexts_in_spans(dim, heads, kv_heads, cap, lens):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch,heads,kv_heads,q_len,causal,cap", [
+    (180, 3, 3, 1, False, 9), (180, 6, 3, 2, True, 150), (100, 3, 3, 1, False, 1600), (150, 4, 2, 3, True, 1400), (40, 2, 2, 9, True, 900), (30, 4, 4, 1, False, 2500)])
+def test_attn_kv4_many_sequences_of_all_lengths(dim, batch, heads, kv_heads, q_len, causal, cap):
+    """Every way a call is cut into waves and spans, with sequences from empty to full side by side."""
+    k, v = kv_rows(batch * cap, kv_heads, dim, cap + batch)
+    c = K.KV4Cache(batch, cap, kv_heads, dim)
+    c.data.fill_(0xFF)
+    lens = torch.randint(0, cap + 1, (batch,), generator=gen(cap)).tolist()
+    lens[0], lens[batch // 2], lens[-1] = cap, 0, 1
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    K.kv4_append(c, k, v, n, n)
+    q = (1.5 * torch.randn(batch * q_len, heads * dim, generator=gen(batch))).to(BF16).cuda()
+    out, lse = K.attn_kv4(q, c, n, heads=heads, scale=dim ** -0.5, q_len=q_len, causal=causal, want_lse=True)
+    check_attn(out, lse, q, k.reshape(batch, cap, -1), v.reshape(batch, cap, -1), heads, kv_heads, dim, batch, q_len, lens, dim ** -0.5, causal)
+
+
 def test_attn_kv4_rising_scores_and_far_apart_maxima():
     """Every tile raises the maximum, by more than the lazy threshold and by less; scores of hundreds."""
     dim, cap = 128, 640
