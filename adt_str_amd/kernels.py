@@ -656,6 +656,11 @@ def _device_of(*tensors) -> int:
     return dev
 
 
+def _ld(t: torch.Tensor) -> int:
+    """Row pitch of a 2-D tensor, the width where it has no second row.  (A broadcast or overlapping one stays what it is, and is refused.)"""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _launch(dev: int, name: str, *args) -> None:
     """``_ffi.call`` with the current stream of device ``dev`` as the last argument, whichever device is current."""
     stream = torch._C._cuda_getCurrentRawStream(dev)      # (torch.cuda.current_stream(dev).cuda_stream without the object: a microsecond)
@@ -673,10 +678,10 @@ def quant_rows_i8(x: torch.Tensor):
     assert x.dtype in (torch.bfloat16, torch.float32) and x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1)
     M, K = x.shape
     dev = _device_of(x)
-    q = torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    q = x.new_empty((M, (K + 15) // 16 * 16), dtype=torch.int8)
+    scale = x.new_empty(M, dtype=torch.float32)
     if M:
-        _launch(dev, "adt_quant_rows_i8", x.data_ptr(), x.dtype == torch.float32, max(x.stride(0), K), M, K, q.data_ptr(), q.shape[1], scale.data_ptr())
+        _launch(dev, "adt_quant_rows_i8", x.data_ptr(), x.dtype == torch.float32, _ld(x), M, K, q.data_ptr(), q.shape[1], scale.data_ptr())
     return q, scale
 
 
@@ -691,10 +696,10 @@ def _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux):
     if residual is not None:
         assert residual.dtype == torch.float32 and residual.dim() == 2 and residual.shape[1] == N and (N == 1 or residual.stride(1) == 1)
         assert res_row_mod >= 0 and residual.shape[0] >= (res_row_mod or M)
-        ep.residual, ep.ld_res, ep.res_row_mod = residual.data_ptr(), max(residual.stride(0), N), res_row_mod
+        ep.residual, ep.ld_res, ep.res_row_mod = residual.data_ptr(), _ld(residual), res_row_mod
     if aux is not None:
         assert out.dtype == torch.float32 and aux.dtype == torch.bfloat16 and aux.shape == (M, N) and (N == 1 or aux.stride(1) == 1)
-        ep.aux_bf16_out, ep.ld_aux = aux.data_ptr(), max(aux.stride(0), N)
+        ep.aux_bf16_out, ep.ld_aux = aux.data_ptr(), _ld(aux)
     return ep
 
 
@@ -710,11 +715,11 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
         assert s.dtype == torch.float32 and s.dim() == 1 and s.numel() == n and s.is_contiguous()
     dev = _device_of(a, a_scale, b, b_scale, out, bias, residual, aux_bf16_out)
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+        out = a.new_empty((M, N), dtype=out_dtype)
     ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
     if M and N:
-        _launch(dev, "adt_gemm_i8", M, N, K, a.data_ptr(), max(a.stride(0), K), a_scale.data_ptr(), b.data_ptr(), max(b.stride(0), K), b_scale.data_ptr(),
-                out.data_ptr(), max(out.stride(0), N), C.byref(ep))
+        _launch(dev, "adt_gemm_i8", M, N, K, a.data_ptr(), _ld(a), a_scale.data_ptr(), b.data_ptr(), _ld(b), b_scale.data_ptr(),
+                out.data_ptr(), _ld(out), C.byref(ep))
     return out
 
 
@@ -730,13 +735,13 @@ def linear_i8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, *, out: 
     assert w_scale.dtype == torch.float32 and w_scale.dim() == 1 and w_scale.numel() == N and w_scale.is_contiguous()
     dev = _device_of(x, w8, w_scale, out, bias, residual, aux_bf16_out)
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        out = x.new_empty((M, N), dtype=out_dtype)
     ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
     if M and N:
         nb = _ffi.load().adt_linear_i8_workspace_bytes(M, K)
-        ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None      # (from the allocator: a captured call gets its graph's own)
-        _launch(dev, "adt_linear_i8", M, N, K, x.data_ptr(), x.dtype == torch.float32, max(x.stride(0), K), w8.data_ptr(), max(w8.stride(0), w8.shape[1]),
-                w_scale.data_ptr(), out.data_ptr(), max(out.stride(0), N), C.byref(ep), ws.data_ptr() if nb else None, nb)
+        ws = x.new_empty(nb, dtype=torch.uint8) if nb else None      # (from the allocator: a captured call gets its graph's own)
+        _launch(dev, "adt_linear_i8", M, N, K, x.data_ptr(), x.dtype == torch.float32, _ld(x), w8.data_ptr(), _ld(w8),
+                w_scale.data_ptr(), out.data_ptr(), _ld(out), C.byref(ep), ws.data_ptr() if nb else None, nb)
     return out
 
 
@@ -760,27 +765,24 @@ class KV4Cache:
         return self.data.numel()
 
 
-def _kv4_rows(cache, end, count, k, v, n):
-    for t in (end, count):
+def _kv4_lengths(cache, *lengths):
+    for t in lengths:
         assert t is None or (t.dtype == torch.int32 and t.dim() == 1 and t.numel() == cache.batch and t.is_contiguous())
-    width = cache.kv_heads * cache.head_dim
-    for t in (k, v):
-        assert t.dim() == 2 and t.shape == (cache.batch * n, width) and t.stride(1) == 1, (t.shape, cache.batch, n, width)
-    return width
 
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, end: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None) -> None:
     """Quantise K and V rows into the cache.  ``k``, ``v``: bf16 ``[batch * n, kv_heads * head_dim]`` (row-strided views allowed), n rows per
     sequence.  Row i < ``count[b]`` (int32, default n) goes to position ``end[b] - count[b] + i`` (``end`` int32: the sequence's length after
     the call, the ``key_len`` of :func:`attn_kv4`; default the capacity); the other rows are left out, as are positions outside the cache."""
-    assert k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16 and k.shape == v.shape
-    if cache.batch == 0 or k.shape[0] == 0:
+    width = cache.kv_heads * cache.head_dim
+    assert k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16 and k.dim() == 2 and k.shape == v.shape and k.stride(1) == 1 and v.stride(1) == 1
+    rows = k.shape[0]
+    if cache.batch == 0 or rows == 0:
         return
-    assert k.shape[0] % cache.batch == 0, (k.shape, cache.batch)
-    n = k.shape[0] // cache.batch
-    width = _kv4_rows(cache, end, count, k, v, n)
+    assert k.shape[1] == width and rows % cache.batch == 0, (k.shape, cache.batch, width)
+    _kv4_lengths(cache, end, count)
     _launch(_device_of(cache.data, k, v, end, count), "adt_kv4_append", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity,
-            k.data_ptr(), max(k.stride(0), width), v.data_ptr(), max(v.stride(0), width), n, end.data_ptr() if end is not None else None,
+            k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), rows // cache.batch, end.data_ptr() if end is not None else None,
             count.data_ptr() if count is not None else None)
 
 
@@ -792,9 +794,9 @@ def kv4_read(cache: KV4Cache, end: Optional[torch.Tensor] = None, count: Optiona
     assert n >= 0
     width = cache.kv_heads * cache.head_dim
     dev = _device_of(cache.data, end, count)
-    k, v = (torch.empty((cache.batch * n, width), dtype=out_dtype, device=cache.data.device) for _ in range(2))
+    k, v = (cache.data.new_empty((cache.batch * n, width), dtype=out_dtype) for _ in range(2))
     if cache.batch and n:
-        _kv4_rows(cache, end, count, k, v, n)
+        _kv4_lengths(cache, end, count)
         _launch(dev, "adt_kv4_read", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity, k.data_ptr(), width, v.data_ptr(), width,
                 out_dtype == torch.float32, n, end.data_ptr() if end is not None else None, count.data_ptr() if count is not None else None)
     return k, v
@@ -813,15 +815,15 @@ def attn_kv4(q: torch.Tensor, cache: KV4Cache, key_len: Optional[torch.Tensor] =
     assert key_len is None or (key_len.dtype == torch.int32 and key_len.dim() == 1 and key_len.numel() == cache.batch and key_len.is_contiguous())
     dev = _device_of(q, cache.data, key_len, out)
     if out is None:
-        out = torch.empty((rows, width), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((rows, width), dtype=torch.bfloat16)
     assert out.dtype == torch.bfloat16 and out.shape == (rows, width) and out.stride(1) == 1
-    lse = torch.empty((cache.batch, heads, q_len), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = q.new_empty((cache.batch, heads, q_len), dtype=torch.float32) if want_lse else None
     if rows:
         d = _ffi.AttnKv4Desc(cache.batch, heads, cache.kv_heads, cache.head_dim, q_len, cache.capacity, causal, scale,
-                             max(q.stride(0), width), max(out.stride(0), width), key_len.data_ptr() if key_len is not None else None)
+                             _ld(q), _ld(out), key_len.data_ptr() if key_len is not None else None)
         ref = C.byref(d)
         nb = _ffi.load().adt_attn_kv4_workspace_bytes(ref)
-        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None       # (from the allocator: a captured call gets its graph's own)
+        ws = q.new_empty(nb, dtype=torch.uint8) if nb else None       # (from the allocator: a captured call gets its graph's own)
         _launch(dev, "adt_attn_kv4", ref, q.data_ptr(), cache.data.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
                 ws.data_ptr() if nb else None, nb)
     return (out, lse) if want_lse else out

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from adt_str_amd import kernels as K
+from adt_str_amd._ffi import AdtError
 
 pytestmark = pytest.mark.gpu
 F32, F64, BF16 = torch.float32, torch.float64, torch.bfloat16
@@ -192,6 +193,21 @@ def test_linear_i8_is_quantise_then_multiply(m, k, dtype):
     assert torch.equal(out, K.gemm_i8(q, s, w8, ws, bias=bias, act=1)) or (m > 2 and torch.equal(out[1:], K.gemm_i8(q, s, w8, ws, bias=bias, act=1)[1:]))
     if m > 2:
         assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
+
+
+def test_few_bits_refuse_rows_that_share_memory():
+    """A broadcast row has pitch 0: read as rows of its width it would run past its memory."""
+    w8, ws = K.quant_rows_i8(torch.randn(32, 64, device="cuda"))
+    row, many = torch.randn(1, 64, device="cuda"), torch.randn(5, 64, device="cuda")
+    q8, s8 = K.quant_rows_i8(many)
+    c = K.KV4Cache(5, 10, 1, 64)
+    kv = many.to(BF16)
+    for call in (lambda: K.quant_rows_i8(row.expand(5, 64)), lambda: K.linear_i8(row.expand(5, 64), w8, ws), lambda: K.gemm_i8(q8[:1].expand(5, 64), s8, w8, ws),
+                 lambda: K.gemm_i8(q8, s8, w8[:1].expand(32, 64), ws), lambda: K.linear_i8(many, w8, ws, residual=torch.zeros(1, 32, device="cuda").expand(5, 32)),
+                 lambda: K.linear_i8(many, w8, ws, out=torch.zeros(1, 32, device="cuda").expand(5, 32)), lambda: K.kv4_append(c, kv, kv[:1].expand(5, 64)),
+                 lambda: K.attn_kv4(kv[:1].expand(5, 64), c, heads=1, scale=1.0)):
+        with pytest.raises(AdtError):
+            call()
 
 
 def test_few_bits_empty_calls():
