@@ -195,6 +195,18 @@ def test_linear_i8_is_quantise_then_multiply(m, k, dtype):
         assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
 
 
+@pytest.mark.parametrize("m,n", [(5, 40), (300, 700), (2100, 1536), (4400, 2304)])
+@pytest.mark.parametrize("act", [0, 1, 2])
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_linear_i8_rows_without_numbers_stay_so_behind_every_activation(m, n, act, out):
+    x = torch.randn(m, 128, generator=gen(m)).cuda()
+    x[m // 2, 7] = math.inf
+    w8, ws = K.quant_rows_i8(torch.randn(n, 128, generator=gen(n)).cuda())
+    y = K.linear_i8(x, w8, ws, act=act, out_dtype=out, residual=torch.ones(m, n, device="cuda"))
+    none = torch.isnan(y)
+    assert none[m // 2].all() and int(none.sum()) == n
+
+
 def test_few_bits_refuse_rows_that_share_memory():
     """A broadcast row has pitch 0: read as rows of its width it would run past its memory."""
     w8, ws = K.quant_rows_i8(torch.randn(32, 64, device="cuda"))
