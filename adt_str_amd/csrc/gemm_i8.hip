@@ -785,8 +785,15 @@ namespace adt {
 // workgroup past 2048 columns (us with 64 / 256 lanes, fp32: 4096 x 4096 17.2 / 14.0, 2048 x 8192 23.1 / 13.9, 1 x 3400 4.1 / 2.6)
 template <bool kF32, int kLanes, int kP>
 static void launch_quant_as(const QuantArgs& a, bool vec, hipStream_t st) {
-  constexpr int kRows = 256 / kLanes;
-  hipLaunchKernelGGL((quant_rows_i8_kernel<kF32, kLanes, kP>), dim3(static_cast<unsigned>((static_cast<long>(a.M) + kRows - 1) / kRows)), dim3(256), 0, st, a, vec);
+  constexpr int64_t kRows = 256 / kLanes, kMost = kRows << 23;      // (a grid holds fewer than 2^32 threads)
+  for (int64_t m0 = 0; m0 < a.M; m0 += kMost) {
+    QuantArgs c = a;
+    c.M = static_cast<int>(std::min(a.M - m0, kMost));
+    c.x = static_cast<const char*>(a.x) + m0 * a.ldx * (kF32 ? 4 : 2);
+    c.q = a.q + m0 * a.ldq;
+    c.scale = a.scale + m0;
+    hipLaunchKernelGGL((quant_rows_i8_kernel<kF32, kLanes, kP>), dim3(static_cast<unsigned>((c.M + kRows - 1) / kRows)), dim3(256), 0, st, c, vec);
+  }
 }
 template <bool kF32>
 static void launch_quant(const QuantArgs& a, bool vec, hipStream_t st) {

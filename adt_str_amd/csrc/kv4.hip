@@ -755,7 +755,7 @@ extern "C" int adt_attn_kv4(const adt_attn_kv4_desc* d, const void* q, const voi
   a.q_len = d->q_len; a.causal = d->causal; a.sl2 = fabsf(d->scale) * 1.4426950408889634f; a.negate = d->scale < 0.f;
   a.rows = p.rows; a.row_blocks = p.row_blocks; a.spans = p.spans; a.span_tiles = p.span_tiles; a.part = static_cast<float*>(ws);
   const int64_t wgs = static_cast<int64_t>(d->batch) * d->kv_heads * p.row_blocks * p.spans, joins = static_cast<int64_t>(d->batch) * d->kv_heads * p.rows;
-  if (wgs > (1LL << 31) - 1 || joins > (1LL << 31) - 1) return set_error(ADT_ESHAPE, "adt_attn_kv4: too many workgroups");
+  if (wgs >= 1LL << 23) return set_error(ADT_ESHAPE, "adt_attn_kv4: too many workgroups");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   typedef int (*Launch)(const KvAttnArgs&, unsigned, hipStream_t);
   static const Launch launches[2][4] = {{launch_attn_kv4<64, 1>, launch_attn_kv4<64, 2>, launch_attn_kv4<64, 4>, launch_attn_kv4<64, 8>},

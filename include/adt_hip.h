@@ -486,7 +486,8 @@ int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, con
  * A group with an infinity or a NaN, or whose range exceeds fp32, stands for NaNs.
  *
  *   adt_kv4_bytes    size of a cache of `capacity` positions per sequence (head_dim 64 or 128); opaque device memory, 16-byte aligned.  It
- *                    need not be cleared: only rows below the lengths that a call names are read.
+ *                    need not be cleared: only rows below the lengths that a call names are read.  Calls on one cache follow one another (one
+ *                    stream, or events): a tile of 32 positions is shared by the appends that fill it.
  *   adt_kv4_append   k, v: bf16 rows, n per sequence (row b * n + i, head h at columns h * head_dim), row strides in elements.  Row i < count[b]
  *                    goes to position end[b] - count[b] + i; count null: n rows, end null: capacity.  Rows i >= count[b], and rows whose position
  *                    lies outside [0, capacity), are left out; every other position keeps what it held.

@@ -65,6 +65,17 @@ def test_quant_rows_ties_extremes_and_rows_without_numbers(dtype):
     assert q[8].abs().max() == 0 and float(s[8]) > 0
 
 
+def test_quant_rows_more_rows_than_one_grid_holds():
+    m = (1 << 27) + 3
+    x = torch.full((m, 1), 2.0, dtype=BF16, device="cuda")
+    x[[0, (1 << 27) - 1, 1 << 27, m - 1], 0] = torch.tensor([-1.0, 4.0, -8.0, 0.0], dtype=BF16, device="cuda")
+    q, s = K.quant_rows_i8(x)
+    picked = [0, 1, (1 << 27) - 1, 1 << 27, m - 2, m - 1]
+    assert q[picked, 0].tolist() == [-127, 127, 127, -127, 127, 0]
+    assert int((q[:, 0] == 127).sum()) == m - 3 and not q[picked, 1:].any()
+    assert torch.equal(s[picked[:5]], torch.tensor([1.0, 2.0, 4.0, 8.0, 2.0], device="cuda") / 127)
+
+
 # --------------------------------------------------------------------------------------------------- products
 def gelu64(z):
     return 0.5 * z * torch.erfc(-z / math.sqrt(2.0))
