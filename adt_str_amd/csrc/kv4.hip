@@ -308,7 +308,7 @@ struct KvAttnArgs {
 };
 constexpr float kKvNegBig = -3.0e38f;               // below every score: the running maximum of a row that has seen no token
 constexpr float kKvThr = 8.0f;
-constexpr int kKvMaxSpans = 64;
+constexpr int kKvMaxSpans = 64, kKvFewSpans = 8;
 
 __device__ __forceinline__ float kv_max_over_groups(float v) {      // over the four lanes that share lane & 15
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -565,15 +565,19 @@ __global__ __launch_bounds__(64 * kW, kW < 8 ? 3 : 1) void attn_kv4_kernel(KvAtt
   }
 }
 
-// One row per workgroup: lane s weighs span s (at most 64 of them); the spans' outputs are dealt to 512 / D threads a channel, all loads at once
-// (a thread a channel: 37 spans 4 us more).
-template <int D>
-__global__ __launch_bounds__(512) void attn_kv4_join_kernel(KvAttnArgs a) {
-  constexpr int kS = 512 / D, kEach = kKvMaxSpans / kS;              // spans s = part_of, part_of + kS, ..: all of a thread's are asked for at once
+// 512 / D / kS rows per workgroup, kS threads a channel: lane s weighs span s (at most 64 of them); the spans' outputs are dealt to the threads of a
+// channel, all loads at once.  kS = 512 / D past eight spans (a thread a channel: 37 spans 4 us more), 1 up to there (1680 rows of 2 spans, 64 channels,
+// 2.2 to 3.9 us; with a workgroup a row 5.0).
+template <int D, int kS>
+__global__ __launch_bounds__(512) void attn_kv4_join_kernel(KvAttnArgs a, int n_rows) {
+  constexpr int kEach = (kS == 1 ? kKvFewSpans : kKvMaxSpans) / kS, kRows = 512 / D / kS;
   __shared__ float so[kS][D];
-  const int orow = blockIdx.x % a.rows, bh = blockIdx.x / a.rows, hk = bh % a.Hk, b = bh / a.Hk;
-  const int lane = threadIdx.x & 63, d = threadIdx.x % D, part_of = threadIdx.x / D;
-  const float* part = a.part + (static_cast<long>(bh) * a.rows + orow) * a.spans * (D + 2);
+  const int lane = threadIdx.x & 63, d = threadIdx.x % D;
+  const int own = __builtin_amdgcn_readfirstlane(threadIdx.x / D), part_of = kS == 1 ? 0 : own;
+  const int row = blockIdx.x * kRows + (kS == 1 ? own : 0);
+  if (row >= n_rows) return;                     // (kS == 1: no barrier below)
+  const int orow = row % a.rows, bh = row / a.rows, hk = bh % a.Hk, b = bh / a.Hk;
+  const float* part = a.part + static_cast<long>(row) * a.spans * (D + 2);
   float ms = kKvNegBig, ls = 0.f, ov[kEach];
   if (lane < a.spans) { ms = part[lane * (D + 2) + D]; ls = part[lane * (D + 2) + D + 1]; }
 #pragma unroll
@@ -593,11 +597,13 @@ __global__ __launch_bounds__(512) void attn_kv4_join_kernel(KvAttnArgs a) {
     const float fs = __shfl(f, part_of + kS * i);
     if (part_of + kS * i < a.spans) ot = fmaf(fs, ov[i], ot);
   }
-  so[part_of][d] = ot;
-  __syncthreads();
-  if (part_of) return;
+  if constexpr (kS > 1) {
+    so[part_of][d] = ot;
+    __syncthreads();
+    if (part_of) return;
 #pragma unroll
-  for (int s = 1; s < kS; ++s) ot += so[s][d];
+    for (int s = 1; s < kS; ++s) ot += so[s][d];
+  }
   const int oi = orow / a.group, oh = hk * a.group + orow % a.group;
   const bool any = lt > 0.f || lt != lt;
   a.out[(static_cast<long>(b) * a.q_len + oi) * a.ldo + oh * D + d] = static_cast<unsigned short>(kv_f2bf(any ? ot / lt : 0.f));
@@ -754,7 +760,7 @@ extern "C" int adt_attn_kv4(const adt_attn_kv4_desc* d, const void* q, const voi
   a.tiles = p.tiles; a.key_len = d->key_len; a.out = static_cast<unsigned short*>(o); a.ldo = d->ldo; a.lse = lse;
   a.q_len = d->q_len; a.causal = d->causal; a.sl2 = fabsf(d->scale) * 1.4426950408889634f; a.negate = d->scale < 0.f;
   a.rows = p.rows; a.row_blocks = p.row_blocks; a.spans = p.spans; a.span_tiles = p.span_tiles; a.part = static_cast<float*>(ws);
-  const int64_t wgs = static_cast<int64_t>(d->batch) * d->kv_heads * p.row_blocks * p.spans, joins = static_cast<int64_t>(d->batch) * d->kv_heads * p.rows;
+  const int64_t wgs = static_cast<int64_t>(d->batch) * d->kv_heads * p.row_blocks * p.spans;
   if (wgs >= 1LL << 23) return set_error(ADT_ESHAPE, "adt_attn_kv4: too many workgroups");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   typedef int (*Launch)(const KvAttnArgs&, unsigned, hipStream_t);
@@ -763,8 +769,11 @@ extern "C" int adt_attn_kv4(const adt_attn_kv4_desc* d, const void* q, const voi
   const Launch launch = launches[d->head_dim == 128][p.waves == 8 ? 3 : p.waves / 2];
   if (int rc = launch(a, static_cast<unsigned>(wgs), st)) return rc;
   if (p.spans > 1) {
-    if (d->head_dim == 128) hipLaunchKernelGGL(attn_kv4_join_kernel<128>, dim3(static_cast<unsigned>(joins)), dim3(512), 0, st, a);
-    else hipLaunchKernelGGL(attn_kv4_join_kernel<64>, dim3(static_cast<unsigned>(joins)), dim3(512), 0, st, a);
+    typedef void (*Join)(KvAttnArgs, int);
+    static const Join join[2][2] = {{attn_kv4_join_kernel<64, 1>, attn_kv4_join_kernel<64, 8>}, {attn_kv4_join_kernel<128, 1>, attn_kv4_join_kernel<128, 4>}};
+    const bool many = p.spans > kKvFewSpans;
+    const int n_rows = static_cast<int>(static_cast<int64_t>(d->batch) * d->kv_heads * p.rows), per_wg = many ? 1 : 512 / d->head_dim;      // (spans: 2^16 rows at most)
+    hipLaunchKernelGGL(join[d->head_dim == 128][many], dim3((n_rows + per_wg - 1) / per_wg), dim3(512), 0, st, a, n_rows);
     ADT_HIP_TRY(hipGetLastError());
   }
   return ADT_OK;
