@@ -116,7 +116,7 @@ SIGNATURES = {
     "adt_embed_bwd_operands_f32": [ptr, ptr, f32, ptr, i64, ptr, i64, i64, i64, ptr, ptr],
     "adt_quant_rows_i8": [ptr, i32, i64, i64, i64, ptr, i64, ptr, ptr],
     "adt_gemm_i8": [i64, i64, i64, ptr, i64, ptr, ptr, i64, ptr, ptr, i64, ptr, ptr],
-    "adt_linear_i8_workspace_bytes": [i64, i64],
+    "adt_linear_i8_workspace_bytes": [i64, i64, i64],
     "adt_linear_i8": [i64, i64, i64, ptr, i32, i64, ptr, i64, ptr, ptr, i64, ptr, ptr, C.c_size_t, ptr],
     "adt_kv4_bytes": [i64, i32, i32, i64],
     "adt_kv4_append": [ptr, i64, i32, i32, i64, ptr, i64, ptr, i64, i64, ptr, ptr, ptr],

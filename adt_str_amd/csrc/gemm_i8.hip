@@ -449,8 +449,8 @@ __global__ __launch_bounds__(kTile == 64 ? 512 : 256) void gemm_i8_kernel(GemmI8
 // ---- few tokens: 16 kMT tokens x 16 channels per workgroup, K dealt in steps of 64 bytes over its eight waves, which join through LDS
 //
 // What bounds such a call is the time of a memory round trip, not its bytes, so a wave asks for the operands of several steps at once and there
-// is one launch where the rows still have to be quantised and are few (kX: x is bf16 or fp32): every workgroup then quantises the
-// rows for itself, 7 instructions a code, from the registers that hold its share of them (K up to 2048).
+// is one launch where the rows still have to be quantised (kX: x is bf16 or fp32): every workgroup then quantises its 16 rows for itself,
+// 7 instructions a code, from the registers that hold its share of them (K up to 2048).
 constexpr int kI8SkinnyDepth = 4, kI8SkinnyWaves = 8;
 struct LinearX { const void* x; long ldx; int K; bool vec; };      // K columns of x; GemmI8Args::K is K rounded up to 16
 enum { kXInt8 = 0, kXBf16 = 1, kXF32 = 2 };
@@ -924,12 +924,17 @@ extern "C" int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64
   return ep->out_fp32 ? launch_i8<true>(g, static_cast<hipStream_t>(stream)) : launch_i8<false>(g, static_cast<hipStream_t>(stream));
 }
 
-// Rows quantised inside the product: up to 16 of them, as long as a workgroup holds them in its registers (us in one launch / in two: 1 x 2304 x 768 3.8 / 5.2,
-// 16 x 2304 x 768 4.1 / 5.6, 16 x 768 x 2048 6.2 / 7.0, 16 x 4096 x 4096 13.4 / 11.7).
-static bool linear_i8_fused(int64_t M, int64_t K) { return M <= 16 && K <= 64 * adt::kI8SkinnyDepth * adt::kI8SkinnyWaves; }
+// Rows quantised inside the product: as long as a workgroup holds its 16 of them in registers, and every workgroup of the card is there for the repeated
+// work of the next 16 channels (us in one launch / in two, bf16 rows: 1 x 2304 x 768 4.0 / 5.4, 64 x 768 x 768 4.2 / 7.0, 64 x 768 x 2048 6.5 / 10.1,
+// 64 x 1400 x 768 5.5 / 7.1, 16 x 8000 x 768 5.8 / 6.4; past two workgroups a CU 64 x 2304 x 768 7.9 / 7.1, 16 x 30000 x 768 17.3 / 8.9).
+static bool linear_i8_fused(int64_t M, int64_t N, int64_t K) {
+  int n_cu = 256;
+  (void)device_cu_count(&n_cu);
+  return K <= 64 * kI8SkinnyDepth * kI8SkinnyWaves && M <= 16 * n_cu && (M + 15) / 16 * ((N + 15) / 16) <= 2 * n_cu;
+}
 
-extern "C" size_t adt_linear_i8_workspace_bytes(int64_t M, int64_t K) {
-  if (M <= 0 || K <= 0 || linear_i8_fused(M, K)) return 0;
+extern "C" size_t adt_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || linear_i8_fused(M, N, K)) return 0;
   return static_cast<size_t>(M) * ((K + 15) / 16 * 16) + static_cast<size_t>(M) * 4;
 }
 
@@ -942,12 +947,12 @@ extern "C" int adt_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int
   const int64_t Kp = (K + 15) / 16 * 16;
   GemmI8Args g = gemm_i8_args(M, N, Kp, W, ldw, w_scale, C, ldc, ep);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (linear_i8_fused(M, K)) {
+  if (linear_i8_fused(M, N, K)) {
     const LinearX lx{x, static_cast<long>(ldx), static_cast<int>(K), aligned16(x) && (ldx * (x_fp32 ? 4 : 2)) % 16 == 0};
     if (ep->out_fp32) return x_fp32 ? launch_i8_skinny<true, 1, kXF32>(g, lx, st) : launch_i8_skinny<true, 1, kXBf16>(g, lx, st);
     return x_fp32 ? launch_i8_skinny<false, 1, kXF32>(g, lx, st) : launch_i8_skinny<false, 1, kXBf16>(g, lx, st);
   }
-  if (!ws || ws_bytes < adt_linear_i8_workspace_bytes(M, K) || !aligned16(ws)) return set_error(ADT_EINVAL, "adt_linear_i8: workspace too small or not 16-byte aligned");
+  if (!ws || ws_bytes < adt_linear_i8_workspace_bytes(M, N, K) || !aligned16(ws)) return set_error(ADT_EINVAL, "adt_linear_i8: workspace too small or not 16-byte aligned");
   float* scale = reinterpret_cast<float*>(static_cast<char*>(ws) + M * Kp);
   if (int rc = adt_quant_rows_i8(x, x_fp32, ldx, M, K, ws, Kp, scale, stream)) return rc;
   g.A = static_cast<const signed char*>(ws); g.lda = Kp; g.a_scale = scale;

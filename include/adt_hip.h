@@ -468,9 +468,9 @@ int adt_gemm_bf16x3(int32_t trans, int64_t M, int64_t N, int64_t K, const void* 
  *                       ep: bias, act, residual (+ res_row_mod), out_fp32, aux_bf16_out (with an fp32 C), as adt_gemm_bf16; alpha must be 1;
  *                       the training fields must be null / 0 (ADT_EINVAL).
  *   adt_linear_i8       both in one call: C = act(x . W^T + bias) + residual for x [M, K] bf16 / fp32 as adt_quant_rows_i8 takes it and W int8 [N, ldw],
- *                       K rounded up to 16 columns, as that leaves it.  Up to 16 rows of 2048 one launch, without a workspace; the same bits either way.
- *                       ws: adt_linear_i8_workspace_bytes(M, K) bytes, 16-byte aligned. */
-size_t adt_linear_i8_workspace_bytes(int64_t M, int64_t K);
+ *                       K rounded up to 16 columns, as that leaves it.  Small products (K <= 2048) are one launch, without a workspace; the same bits either way.
+ *                       ws: adt_linear_i8_workspace_bytes(M, N, K) bytes, 16-byte aligned. */
+size_t adt_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int adt_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int32_t x_fp32, int64_t ldx, const void* W, int64_t ldw, const float* w_scale,
                   void* C, int64_t ldc, const adt_gemm_epilogue* ep, void* ws, size_t ws_bytes, void* stream);
 int adt_quant_rows_i8(const void* x, int32_t x_fp32, int64_t ldx, int64_t M, int64_t K, void* q, int64_t ldq, float* scale, void* stream);

@@ -190,7 +190,7 @@ def test_gemm_i8_sums_stay_exact_at_the_longest_k():
     assert out[0].tolist() == [float(torch.tensor(-127 * 127 * k, dtype=F32)), float(torch.tensor(127 * 127 * k - 127, dtype=F32))]
 
 
-@pytest.mark.parametrize("m", [1, 16, 40, 64, 65, 900])
+@pytest.mark.parametrize("m", [1, 16, 40, 64, 65, 500, 900])
 @pytest.mark.parametrize("k", [50, 768, 2300])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_linear_i8_is_quantise_then_multiply(m, k, dtype):
