@@ -728,7 +728,8 @@ def linear_i8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, *, out: 
               aux_bf16_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [M, K]`` (bf16 / fp32, row-strided views allowed) through a linear layer whose weights are int8 with one scale per output channel
     (``w8, w_scale = quant_rows_i8(weight)``): the rows are quantised (``quant_rows_i8``) and multiplied (``gemm_i8``) in one call
-    (``adt_linear_i8``), small products in one launch; the same bits as the two."""
+    (``adt_linear_i8``), small products in one launch; the same bits as the two.
+    ``out`` shares no memory with ``x``; ``residual`` may be ``out``."""
     assert x.dtype in (torch.bfloat16, torch.float32) and x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1)
     assert w8.dtype == torch.int8 and w8.dim() == 2 and w8.stride(1) == 1 and w8.shape[1] == (x.shape[1] + 15) // 16 * 16, (x.shape, w8.shape)
     (M, K), N = x.shape, w8.shape[0]

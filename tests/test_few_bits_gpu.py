@@ -167,6 +167,24 @@ def test_gemm_i8_odd_widths_activation_residual_and_what_lies_around(m, n, k, ou
             assert torch.equal(copy[:, lo:lo + n], o.to(BF16)) and (copy[:, :lo] == 7).all() and (copy[:, lo + n:] == 7).all()
 
 
+def test_few_bits_offsets_past_32_bits():
+    m, n, k = 70001, 32768, 48                                                # 2.3e9 results
+    g = gen(5)
+    x = torch.randn(m, k, generator=g).cuda()
+    w8, ws = K.quant_rows_i8(torch.randn(n, k, generator=g).cuda())
+    q, s = K.quant_rows_i8(x)
+    out = K.linear_i8(x, w8, ws)
+    for r in (0, 65535, 65537, m - 1):
+        check_product(q[r:r + 1], s[r:r + 1], w8, ws, out[r:r + 1])
+    del out
+    rows = 540000
+    x = torch.ones(1, 4096, dtype=BF16, device="cuda").repeat(rows, 1)        # 2.2e9 values
+    x[-1] = -2.0
+    x[-1, 5] = 4.0
+    q, s = K.quant_rows_i8(x)
+    assert int(q[-1, 5]) == 127 and int(q[-1, 4]) == -64 and float(s[-1]) == float(torch.tensor(4.0) / 127) and bool((q[-2] == 127).all())
+
+
 @pytest.mark.parametrize("m,n,k", [(7, 40, 64), (300, 776, 768), (1300, 2264, 144), (5000, 2304, 768)])
 def test_gemm_i8_adds_to_the_residual_in_place(m, n, k):
     g = gen(m * n)
@@ -555,3 +573,19 @@ def test_few_bits_on_another_stream_and_in_graphs():
             assert torch.equal(step(x), want)
             junk = torch.randn(1 << 20, device="cuda").sum()
             del junk
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 300, 200), (300, 700, 2500), (1300, 2264, 144), (4400, 2304, 768)])
+def test_linear_i8_of_every_size_replays_as_a_graph(m, n, k):
+    g = gen(n)
+    w8, ws = K.quant_rows_i8(torch.randn(n, k, generator=g).cuda())
+    x = torch.randn(m, k, generator=g).cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.linear_i8(x, w8, ws, act=1)
+    for rep in range(3):
+        x.copy_(torch.randn(m, k, generator=g))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, K.linear_i8(x, w8, ws, act=1))
