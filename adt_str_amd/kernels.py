@@ -664,7 +664,7 @@ def _ld(t: torch.Tensor) -> int:
 def _launch(dev: int, name: str, *args) -> None:
     """``_ffi.call`` with the current stream of device ``dev`` as the last argument, whichever device is current."""
     stream = torch._C._cuda_getCurrentRawStream(dev)      # (torch.cuda.current_stream(dev).cuda_stream without the object: a microsecond)
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         _ffi.call(name, *args, stream)
     else:
         with torch.cuda.device(dev):
@@ -685,11 +685,19 @@ def quant_rows_i8(x: torch.Tensor):
     return q, scale
 
 
+def _i8_out(like, M, N, out, out_dtype):
+    """``out`` if it can hold the results, or a new tensor -> it and its row pitch."""
+    if out is None:
+        assert out_dtype in (torch.bfloat16, torch.float32)
+        return like.new_empty((M, N), dtype=out_dtype), N
+    assert out.shape == (M, N) and out.dtype in (torch.bfloat16, torch.float32) and (N <= 1 or out.stride(1) == 1)
+    return out, _ld(out)
+
+
 def _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux):
     assert act in (0, 1, 2)
-    assert out.shape == (M, N) and out.dtype in (torch.bfloat16, torch.float32) and (N <= 1 or out.stride(1) == 1)
     ep = _ffi.GemmEpilogue()
-    ep.alpha, ep.act, ep.out_fp32 = 1.0, act, int(out.dtype == torch.float32)
+    ep.alpha, ep.act, ep.out_fp32 = 1.0, act, out.dtype == torch.float32
     if bias is not None:
         assert bias.dtype == torch.float32 and bias.numel() == N and bias.is_contiguous()
         ep.bias = bias.data_ptr()
@@ -708,18 +716,17 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
             act: int = 0, aux_bf16_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act((a [M, K] @ b [N, K].T) * a_scale[:, None] * b_scale + bias) + residual`` with int8 operands and exact integer sums (``adt_gemm_i8``):
     the inference epilogue of :func:`gemm`.  ``K`` is a multiple of 16 (``quant_rows_i8`` pads), at most 131072."""
-    assert a.dtype == torch.int8 and b.dtype == torch.int8 and a.dim() == 2 and b.dim() == 2 and a.shape[1] == b.shape[1]
-    (M, K), N = a.shape, b.shape[0]
-    assert K > 0 and K % 16 == 0 and a.stride(1) == 1 and b.stride(1) == 1
+    assert a.dtype == torch.int8 and b.dtype == torch.int8 and a.dim() == 2 and b.dim() == 2
+    (M, K), (N, Kb), (lda, one_a), (ldb, one_b) = a.shape, b.shape, a.stride(), b.stride()
+    assert K == Kb and K > 0 and K % 16 == 0 and one_a == 1 and one_b == 1, (a.shape, b.shape)
     for s, n in ((a_scale, M), (b_scale, N)):
         assert s.dtype == torch.float32 and s.dim() == 1 and s.numel() == n and s.is_contiguous()
     dev = _device_of(a, a_scale, b, b_scale, out, bias, residual, aux_bf16_out)
-    if out is None:
-        out = a.new_empty((M, N), dtype=out_dtype)
+    out, ldo = _i8_out(a, M, N, out, out_dtype)
     ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
     if M and N:
-        _launch(dev, "adt_gemm_i8", M, N, K, a.data_ptr(), _ld(a), a_scale.data_ptr(), b.data_ptr(), _ld(b), b_scale.data_ptr(),
-                out.data_ptr(), _ld(out), C.byref(ep))
+        _launch(dev, "adt_gemm_i8", M, N, K, a.data_ptr(), lda if M > 1 else K, a_scale.data_ptr(), b.data_ptr(), ldb if N > 1 else K, b_scale.data_ptr(),
+                out.data_ptr(), ldo, C.byref(ep))
     return out
 
 
@@ -730,19 +737,19 @@ def linear_i8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, *, out: 
     (``w8, w_scale = quant_rows_i8(weight)``): the rows are quantised (``quant_rows_i8``) and multiplied (``gemm_i8``) in one call
     (``adt_linear_i8``), small products in one launch; the same bits as the two.
     ``out`` shares no memory with ``x``; ``residual`` may be ``out``."""
-    assert x.dtype in (torch.bfloat16, torch.float32) and x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1)
-    assert w8.dtype == torch.int8 and w8.dim() == 2 and w8.stride(1) == 1 and w8.shape[1] == (x.shape[1] + 15) // 16 * 16, (x.shape, w8.shape)
-    (M, K), N = x.shape, w8.shape[0]
+    assert x.dim() == 2 and w8.dim() == 2 and w8.dtype == torch.int8
+    (M, K), (N, Kw), (ldx, one_x), (ldw, one_w), kind = x.shape, w8.shape, x.stride(), w8.stride(), x.dtype
+    assert (kind == torch.bfloat16 or kind == torch.float32) and K > 0 and (one_x == 1 or K == 1)
+    assert one_w == 1 and Kw == (K + 15) // 16 * 16, (x.shape, w8.shape)
     assert w_scale.dtype == torch.float32 and w_scale.dim() == 1 and w_scale.numel() == N and w_scale.is_contiguous()
     dev = _device_of(x, w8, w_scale, out, bias, residual, aux_bf16_out)
-    if out is None:
-        out = x.new_empty((M, N), dtype=out_dtype)
+    out, ldo = _i8_out(x, M, N, out, out_dtype)
     ep = _i8_epilogue(M, N, out, bias, residual, res_row_mod, act, aux_bf16_out)
     if M and N:
         nb = _ffi.load().adt_linear_i8_workspace_bytes(M, N, K)
         ws = x.new_empty(nb, dtype=torch.uint8) if nb else None      # (from the allocator: a captured call gets its graph's own)
-        _launch(dev, "adt_linear_i8", M, N, K, x.data_ptr(), x.dtype == torch.float32, _ld(x), w8.data_ptr(), _ld(w8),
-                w_scale.data_ptr(), out.data_ptr(), _ld(out), C.byref(ep), ws.data_ptr() if nb else None, nb)
+        _launch(dev, "adt_linear_i8", M, N, K, x.data_ptr(), kind == torch.float32, ldx if M > 1 else K, w8.data_ptr(), ldw if N > 1 else Kw,
+                w_scale.data_ptr(), out.data_ptr(), ldo, C.byref(ep), ws.data_ptr() if nb else None, nb)
     return out
 
 
@@ -775,31 +782,32 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, end: Optional[
     """Quantise K and V rows into the cache.  ``k``, ``v``: bf16 ``[batch * n, kv_heads * head_dim]`` (row-strided views allowed), n rows per
     sequence.  Row i < ``count[b]`` (int32, default n) goes to position ``end[b] - count[b] + i`` (``end`` int32: the sequence's length after
     the call, the ``key_len`` of :func:`attn_kv4`; default the capacity); the other rows are left out, as are positions outside the cache."""
-    width = cache.kv_heads * cache.head_dim
-    assert k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16 and k.dim() == 2 and k.shape == v.shape and k.stride(1) == 1 and v.stride(1) == 1
-    rows = k.shape[0]
-    if cache.batch == 0 or rows == 0:
+    batch, heads, dim = cache.batch, cache.kv_heads, cache.head_dim
+    assert k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16 and k.dim() == 2 and v.dim() == 2
+    (rows, width), (ldk, one_k), (ldv, one_v) = k.shape, k.stride(), v.stride()
+    assert v.shape == (rows, width) and one_k == 1 and one_v == 1
+    if batch == 0 or rows == 0:
         return
-    assert k.shape[1] == width and rows % cache.batch == 0, (k.shape, cache.batch, width)
+    assert width == heads * dim and rows % batch == 0, (k.shape, batch, heads, dim)
     _kv4_lengths(cache, end, count)
-    _launch(_device_of(cache.data, k, v, end, count), "adt_kv4_append", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity,
-            k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), rows // cache.batch, end.data_ptr() if end is not None else None,
-            count.data_ptr() if count is not None else None)
+    _launch(_device_of(cache.data, k, v, end, count), "adt_kv4_append", cache.data.data_ptr(), batch, heads, dim, cache.capacity,
+            k.data_ptr(), ldk if rows > 1 else width, v.data_ptr(), ldv if rows > 1 else width, rows // batch,
+            None if end is None else end.data_ptr(), None if count is None else count.data_ptr())
 
 
 def kv4_read(cache: KV4Cache, end: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None, n: Optional[int] = None, out_dtype=torch.bfloat16):
     """The rows that ``kv4_append(cache, k, v, end, count)`` with n rows per sequence would write, as the values the cache holds ->
     ``(k, v) [batch * n, kv_heads * head_dim]`` in bf16 or fp32 (default: the whole capacity); rows i >= ``count[b]`` are zeros."""
-    assert out_dtype in (torch.bfloat16, torch.float32)
-    n = cache.capacity if n is None else int(n)
+    assert out_dtype == torch.bfloat16 or out_dtype == torch.float32
+    data, batch, heads, dim = cache.data, cache.batch, cache.kv_heads, cache.head_dim
+    n, width = cache.capacity if n is None else int(n), heads * dim
     assert n >= 0
-    width = cache.kv_heads * cache.head_dim
-    dev = _device_of(cache.data, end, count)
-    k, v = (cache.data.new_empty((cache.batch * n, width), dtype=out_dtype) for _ in range(2))
-    if cache.batch and n:
+    dev = _device_of(data, end, count)
+    k, v = data.new_empty((batch * n, width), dtype=out_dtype), data.new_empty((batch * n, width), dtype=out_dtype)
+    if batch and n:
         _kv4_lengths(cache, end, count)
-        _launch(dev, "adt_kv4_read", cache.data.data_ptr(), cache.batch, cache.kv_heads, cache.head_dim, cache.capacity, k.data_ptr(), width, v.data_ptr(), width,
-                out_dtype == torch.float32, n, end.data_ptr() if end is not None else None, count.data_ptr() if count is not None else None)
+        _launch(dev, "adt_kv4_read", data.data_ptr(), batch, heads, dim, cache.capacity, k.data_ptr(), width, v.data_ptr(), width,
+                out_dtype == torch.float32, n, None if end is None else end.data_ptr(), None if count is None else count.data_ptr())
     return k, v
 
 
@@ -809,22 +817,24 @@ def attn_kv4(q: torch.Tensor, cache: KV4Cache, key_len: Optional[torch.Tensor] =
     (int32, default the capacity) -> ``o [batch * q_len, heads * head_dim]`` bf16, with ``want_lse`` also the log-sum-exp rows fp32
     ``[batch, heads, q_len]``.  ``heads`` is a multiple of the cache's ``kv_heads`` (grouped heads).  ``causal``: the queries are the sequence's
     last ``q_len`` positions, query i sees ``key_len[b] - (q_len - 1 - i)`` of them.  A query that sees none gets zeros (lse -inf)."""
-    width = heads * cache.head_dim
-    rows = cache.batch * q_len
-    assert q.dtype == torch.bfloat16 and q.dim() == 2 and q.stride(1) == 1 and q_len > 0 and heads > 0 and heads % cache.kv_heads == 0
-    assert q.shape[0] == rows and q.shape[1] >= width, (q.shape, rows, width)
-    assert key_len is None or (key_len.dtype == torch.int32 and key_len.dim() == 1 and key_len.numel() == cache.batch and key_len.is_contiguous())
-    dev = _device_of(q, cache.data, key_len, out)
+    data, batch, kv_heads, dim = cache.data, cache.batch, cache.kv_heads, cache.head_dim
+    width, rows = heads * dim, batch * q_len
+    assert q.dtype == torch.bfloat16 and q.dim() == 2 and q_len > 0 and heads > 0 and heads % kv_heads == 0
+    (q_rows, q_width), (ldq, one_q) = q.shape, q.stride()
+    assert q_rows == rows and q_width >= width and one_q == 1, (q.shape, rows, width)
+    assert key_len is None or (key_len.dtype == torch.int32 and key_len.dim() == 1 and key_len.numel() == batch and key_len.is_contiguous())
+    dev = _device_of(q, data, key_len, out)
     if out is None:
-        out = q.new_empty((rows, width), dtype=torch.bfloat16)
-    assert out.dtype == torch.bfloat16 and out.shape == (rows, width) and out.stride(1) == 1
-    lse = q.new_empty((cache.batch, heads, q_len), dtype=torch.float32) if want_lse else None
+        out, ldo = q.new_empty((rows, width)), width
+    else:
+        assert out.dtype == torch.bfloat16 and out.shape == (rows, width) and out.stride(1) == 1
+        ldo = _ld(out)
+    lse = q.new_empty((batch, heads, q_len), dtype=torch.float32) if want_lse else None
     if rows:
-        d = _ffi.AttnKv4Desc(cache.batch, heads, cache.kv_heads, cache.head_dim, q_len, cache.capacity, causal, scale,
-                             _ld(q), _ld(out), key_len.data_ptr() if key_len is not None else None)
-        ref = C.byref(d)
+        ref = C.byref(_ffi.AttnKv4Desc(batch, heads, kv_heads, dim, q_len, cache.capacity, causal, scale, ldq if rows > 1 else q_width, ldo,
+                                       None if key_len is None else key_len.data_ptr()))
         nb = _ffi.load().adt_attn_kv4_workspace_bytes(ref)
         ws = q.new_empty(nb, dtype=torch.uint8) if nb else None       # (from the allocator: a captured call gets its graph's own)
-        _launch(dev, "adt_attn_kv4", ref, q.data_ptr(), cache.data.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
+        _launch(dev, "adt_attn_kv4", ref, q.data_ptr(), data.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
                 ws.data_ptr() if nb else None, nb)
     return (out, lse) if want_lse else out
