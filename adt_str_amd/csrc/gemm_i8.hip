@@ -887,15 +887,15 @@ static int launch_i8(const GemmI8Args& g, hipStream_t st) {
   const bool extra = g.residual || g.aux;
   const int form = g.act == 0 ? (extra ? kI8Residual : kI8Plain) : (g.act == 1 && !extra ? kI8Gelu : kI8Any);
   const int64_t tm = (g.M + 127) / 128, tn = (g.N + 127) / 128, bm = (g.M + 255) / 256, bn = (g.N + 255) / 256, sm = (g.M + 63) / 64, sn = (g.N + 63) / 64;
-  // Few tokens: the kernel that asks for everything at once, while its workgroups of up to 64 tokens x 16 channels are one a CU, or two where they hold
-  // no more than 32 tokens; then 64 x 64 tiles while they are two a CU at most (us with 16 channels / 64 x 64 / 128 x 128 tiles: 200 x 1000 x 1000
-  // 4.0 / 5.0 / 9.2, 16 x 8000 x 768 3.7 / 4.7 / 7.5, 32 x 16000 x 768 7.3 / 4.8 / 7.7, 128 x 2304 x 768 6.2 / 4.7 / 8.0, 1024 x 768 x 768 8.8 / 4.9 / 8.0,
-  // 256 x 4096 x 4096 40 / 13.3 / 25.6; three tiles a CU, 1282 x 2263 x 137, 14.2 / 8.6 / 7.6).
-  if (sm * ((g.N + 15) / 16) <= (g.M <= 32 ? 2 : 1) * n_cu) {
-    if (g.M <= 16) return launch_i8_skinny<kOut32, 1, kXInt8>(g, LinearX{}, st);
-    if (g.M <= 32) return launch_i8_skinny<kOut32, 2, kXInt8>(g, LinearX{}, st);
-    return launch_i8_skinny<kOut32, 4, kXInt8>(g, LinearX{}, st);
-  }
+  // Few tokens: the kernel that asks for everything at once, with 16, 32 or 64 tokens a workgroup, the fewest that leave one workgroup of 16 channels a CU,
+  // or two where 32 are all there are; then 64 x 64 tiles while they are two a CU at most (us with 16 tokens / 32 / 64 / 64 x 64 tiles / 128 x 128:
+  // 64 x 768 x 768 3.0 / 3.4 / 4.2 / -, 128 x 768 x 3000 5.7 / 5.0 / 6.7 / -, 64 x 4096 x 4096 17 / 13.4 / 11.9 / 10.5, 16 x 8000 x 768 3.7 / - / - / 4.7 / 7.5,
+  // 32 x 16000 x 768 - / 7.3 / - / 4.8 / 7.7, 128 x 2304 x 768 - / - / 6.2 / 4.7 / 8.0, 256 x 4096 x 4096 - / - / 40 / 13.3 / 25.6;
+  // three 64 x 64 tiles a CU, 1282 x 2263 x 137, 8.6 / 7.6).
+  const int64_t cols = (g.N + 15) / 16;
+  if ((g.M + 15) / 16 * cols <= (g.M <= 16 ? 2 : 1) * n_cu) return launch_i8_skinny<kOut32, 1, kXInt8>(g, LinearX{}, st);
+  if ((g.M + 31) / 32 * cols <= (g.M <= 32 ? 2 : 1) * n_cu) return launch_i8_skinny<kOut32, 2, kXInt8>(g, LinearX{}, st);
+  if (sm * cols <= n_cu) return launch_i8_skinny<kOut32, 4, kXInt8>(g, LinearX{}, st);
   if (sm * sn <= 2 * n_cu) return launch_i8_tile<kOut32, 64, 4>(g, form, sm, sn, st);
   // 256 x 256 tiles run one per CU and twice as efficiently, but in whole rounds: a round of them costs 1.6 of 128 x 128 ones at two per CU (us with
   // 256 / 128: 4096 x 2304 x 768 16.4 / 18.9, 7747 x 768 x 768 14.6 / 11.2, 8192 x 2304 x 768 29.4 / 29.3, 16384 x 2304 x 768 43.6 / 53.1,
