@@ -764,9 +764,9 @@ extern "C" int adt_attn_kv4(const adt_attn_kv4_desc* d, const void* q, const voi
   if (wgs >= 1LL << 23) return set_error(ADT_ESHAPE, "adt_attn_kv4: too many workgroups");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   typedef int (*Launch)(const KvAttnArgs&, unsigned, hipStream_t);
-  static const Launch launches[2][4] = {{launch_attn_kv4<64, 1>, launch_attn_kv4<64, 2>, launch_attn_kv4<64, 4>, launch_attn_kv4<64, 8>},
-                                        {launch_attn_kv4<128, 1>, launch_attn_kv4<128, 2>, launch_attn_kv4<128, 4>, launch_attn_kv4<128, 8>}};
-  const Launch launch = launches[d->head_dim == 128][p.waves == 8 ? 3 : p.waves / 2];
+  static const Launch launches[2][3] = {{launch_attn_kv4<64, 2>, launch_attn_kv4<64, 4>, launch_attn_kv4<64, 8>},
+                                        {launch_attn_kv4<128, 2>, launch_attn_kv4<128, 4>, launch_attn_kv4<128, 8>}};
+  const Launch launch = launches[d->head_dim == 128][p.waves >> 2];
   if (int rc = launch(a, static_cast<unsigned>(wgs), st)) return rc;
   if (p.spans > 1) {
     typedef void (*Join)(KvAttnArgs, int);
