@@ -393,9 +393,11 @@ __global__ __launch_bounds__(64 * kW, kW < 8 ? 3 : 1) void attn_kv4_kernel(KvAtt
   int tile = span * a.span_tiles + wave;
   load_k(min(tile, a.tiles - 1));
   load_v(min(tile, a.tiles - 1));
-  klen = klen < 0 ? 0 : (klen > a.cap ? a.cap : klen);
-  const int qlast = min(rb * 16 + 15, a.rows - 1) / a.group;
-  const int most = a.causal ? klen - (a.q_len - 1 - qlast) : klen;   // the tokens that some row of this block sees
+  // Query i of a causal call sees klen - (q_len - 1 - i) positions, of which the cache has the first cap: a length past the capacity is taken to the
+  // capacity behind the subtraction, not in front of it.
+  klen = max(klen, 0);
+  auto seen = [&](int row) { return min(a.causal ? klen - (a.q_len - 1 - row / a.group) : klen, a.cap); };
+  const int most = seen(min(rb * 16 + 15, a.rows - 1));              // the tokens that some row of this block sees
   const int tile_end = min((max(most, 0) + kKvTile - 1) / kKvTile, (span + 1) * a.span_tiles);
 
   unsigned short* const ql = reinterpret_cast<unsigned short*>(so);  // [16][D + 8]
@@ -424,8 +426,8 @@ __global__ __launch_bounds__(64 * kW, kW < 8 ? 3 : 1) void attn_kv4_kernel(KvAtt
   for (int g = 0; g < kG; ++g) qs[g] = kv_sum_over_groups(qs[g]);
   __syncthreads();                                                   // ql becomes so
   // this lane's row (as a column of the score product) sees the tokens [0, limit)
-  const int limit = a.causal ? klen - (a.q_len - 1 - min(rb * 16 + li, a.rows - 1) / a.group) : klen;
-  const int least = a.causal ? klen - (a.q_len - 1) : klen;
+  const int limit = seen(min(rb * 16 + li, a.rows - 1));
+  const int least = seen(0);
 
   unsigned mask = 0x000f000fu, bits = 0x43004300u;
   asm volatile("" : "+v"(mask), "+s"(bits));

@@ -816,7 +816,8 @@ def attn_kv4(q: torch.Tensor, cache: KV4Cache, key_len: Optional[torch.Tensor] =
     """Attention of ``q [batch * q_len, >= heads * head_dim]`` (bf16, row-strided views allowed) over the cache's first ``key_len[b]`` positions
     (int32, default the capacity) -> ``o [batch * q_len, heads * head_dim]`` bf16, with ``want_lse`` also the log-sum-exp rows fp32
     ``[batch, heads, q_len]``.  ``heads`` is a multiple of the cache's ``kv_heads`` (grouped heads).  ``causal``: the queries are the sequence's
-    last ``q_len`` positions, query i sees ``key_len[b] - (q_len - 1 - i)`` of them.  A query that sees none gets zeros (lse -inf)."""
+    last ``q_len`` positions, query i sees the first ``key_len[b] - (q_len - 1 - i)``; a length may exceed the capacity, and what lies behind
+    it is seen by nobody.  A query that sees none gets zeros (lse -inf)."""
     data, batch, kv_heads, dim = cache.data, cache.batch, cache.kv_heads, cache.head_dim
     width, rows = heads * dim, batch * q_len
     assert q.dtype == torch.bfloat16 and q.dim() == 2 and q_len > 0 and heads > 0 and heads % kv_heads == 0

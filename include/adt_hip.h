@@ -496,7 +496,8 @@ int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, con
  *   adt_attn_kv4     o = softmax(q k^T * scale) v over the positions below key_len[b] (null: capacity), q and o bf16 [batch * q_len, >= heads *
  *                    head_dim].  heads is a multiple of kv_heads: query heads g * kv_head .. + g - 1 read K/V head kv_head (g = heads / kv_heads).
  *                    causal: query i sees the positions below key_len[b] - (q_len - 1 - i), that is, the queries are the sequence's last
- *                    positions.  A query that sees no position gets zeros (lse -inf).  lse: optional fp32 [batch, heads, q_len]. */
+ *                    positions.  Of a sequence that is longer than the capacity the cache has the first `capacity` positions, and a query sees
+ *                    those of its own that are among them.  A query that sees no position gets zeros (lse -inf).  lse: optional fp32 [batch, heads, q_len]. */
 size_t adt_kv4_bytes(int64_t batch, int32_t kv_heads, int32_t head_dim, int64_t capacity);
 int adt_kv4_append(void* cache, int64_t batch, int32_t kv_heads, int32_t head_dim, int64_t capacity, const void* k, int64_t ldk, const void* v,
                    int64_t ldv, int64_t n, const int32_t* end, const int32_t* count, void* stream);
