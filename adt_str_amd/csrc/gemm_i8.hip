@@ -49,7 +49,10 @@ __device__ __forceinline__ float i8_relu(float x) { return x < 0.f ? 0.f : x; } 
 // 16 to 256 lanes per row.  The codes are those of real arithmetic: with e the exponent of a, n = x 127 2^-e is exact for bf16 x (and carried with
 // its rounding error for fp32 x), b = a 2^-e lies in [1, 2), and n / b is formed as r0 = n y, y = 1 / b, corrected by the exact remainder
 // fma(-r0, b, n): a correctly rounded quotient, so that x = a / 2 is 63.5 and not a neighbour of it.  Rounding to the integer is the
-// addition of 1.5 2^23, whose low byte is then the code.
+// addition of 1.5 2^23, whose low byte is then the code.  A bf16 x has no quotient within 2^-16 of a half that is none (2 n and an odd multiple of b are
+// multiples of 2^-14 at least); an fp32 x has, and its quotient as a float may be a half that it is not.  An element with a quotient that near a half
+// in one of the wave's rows is therefore coded again by the sign of an exact difference (quant_code_exact): about one in a thousand (4096 x 4096 in
+// fp32 14.2 us, without the second look 13.9 and 1.6e-6 of the codes wrong by one).
 // Bound: the memory, a row is read once and held (63104 x 768 bf16 24.5 us, 6 TB/s with the codes, part of it from the last-level cache).
 struct QuantArgs { const void* x; long ldx; signed char* q; long ldq; float* scale; int M, K, Kp; };
 constexpr float kQuantTiny = 7.888609052210118e-31f;      // 2^-100
@@ -67,14 +70,41 @@ __device__ __forceinline__ RowScale row_scale(unsigned abits, float* scale) {   
   *scale = s.bad ? __uint_as_float(0x7fc00000u) : __uint_as_float(a) / 127.0f;
   return s;
 }
-template <bool kF32>
-__device__ __forceinline__ unsigned quant_code(float x, const RowScale& s) {
-  const float n = x * s.c;
-  const float r0 = n * s.y;
-  float rem = fmaf(-r0, s.b, n);
-  if (kF32) rem += fmaf(x, s.c, -n);
-  const float r = fmaf(rem, s.y, r0);
-  return __float_as_uint(r + 12582912.0f);
+constexpr float kQuantRound = 12582912.0f;                     // 1.5 2^23
+// k = an integer within one half and a few roundings of the quotient: n - k b is then a float (a multiple of 2^-23 below 1 + 2^-14), and so is its distance
+// from b / 2 where that is small; with n's rounding error e1 added, the sum's sign is the sign of |x 127 / a - k| - 1/2.
+__device__ __forceinline__ unsigned quant_code_exact(float x, const RowScale& s) {
+  const float n = x * s.c, e1 = fmaf(x, s.c, -n);
+  const float t = fmaf(n, s.y, kQuantRound);
+  const float d = fmaf(-(t - kQuantRound), s.b, n);
+  const float past = (fabsf(d) - 0.5f * s.b) + (d < 0.f ? -e1 : e1);
+  const unsigned k = __float_as_uint(t);
+  return past > 0.f || (past == 0.f && (k & 1u)) ? k + (d < 0.f ? -1 : 1) : k;
+}
+template <bool kF32, int kN>
+__device__ __forceinline__ void quant_codes(const float (&x)[kN], const RowScale& s, unsigned (&q)[kN]) {
+  float off[kN], most = 0.f;                                   // distances of the quotients from their integers
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const float n = x[j] * s.c;
+    const float r0 = n * s.y;
+    float rem = fmaf(-r0, s.b, n);
+    if (kF32) rem += fmaf(x[j], s.c, -n);
+    const float r = fmaf(rem, s.y, r0), t = r + kQuantRound;
+    q[j] = __float_as_uint(t);
+    if (kF32) {
+      off[j] = fabsf(r - (t - kQuantRound));
+      most = fmaxf(most, off[j]);
+    }
+  }
+  if constexpr (kF32) {
+    constexpr float kNear = 0.5f - 0x1p-17f;                   // (a quotient is off by half of 2^-17, its last rounding, and 2^-38)
+    if (__builtin_amdgcn_ballot_w64(most > kNear) != 0) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+        if (__builtin_amdgcn_ballot_w64(off[j] > kNear) != 0) q[j] = quant_code_exact(x[j], s);
+    }
+  }
 }
 __device__ __forceinline__ unsigned pack_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {      // the low bytes
   const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
@@ -126,8 +156,7 @@ __device__ __forceinline__ unsigned widest8(const float (&v)[8], unsigned mx) {
 template <bool kF32>
 __device__ __forceinline__ uint2 quant8(const float (&v)[8], const RowScale& s) {
   unsigned q[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = quant_code<kF32>(v[j], s);
+  quant_codes<kF32>(v, s, q);
   return s.bad ? make_uint2(0u, 0u) : make_uint2(pack_bytes(q[0], q[1], q[2], q[3]), pack_bytes(q[4], q[5], q[6], q[7]));
 }
 // kLanes lanes per row, kP pieces of eight elements per lane held in registers from the maximum to the codes: one read of x.  kP = 0: any K,
@@ -542,12 +571,10 @@ __global__ __launch_bounds__(64 * kI8SkinnyWaves) void gemm_i8_skinny_kernel(Gem
     const RowScale rs = row_scale(mx, &a_own);
     auto codes = [&](const float (&v)[16]) {
       i32x4 f;
+      unsigned c[16];
+      quant_codes<kX == kXF32>(v, rs, c);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned w = pack_bytes(quant_code<kX == kXF32>(v[4 * q], rs), quant_code<kX == kXF32>(v[4 * q + 1], rs), quant_code<kX == kXF32>(v[4 * q + 2], rs),
-                                      quant_code<kX == kXF32>(v[4 * q + 3], rs));
-        f[q] = rs.bad ? 0 : static_cast<int>(w);
-      }
+      for (int q = 0; q < 4; ++q) f[q] = rs.bad ? 0 : static_cast<int>(pack_bytes(c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]));
       return f;
     };
 #pragma unroll

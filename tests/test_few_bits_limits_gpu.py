@@ -8,9 +8,48 @@ from adt_str_amd import kernels as K
 from tests.test_few_bits_gpu import check_attn, check_held, gen, kv_rows
 
 pytestmark = pytest.mark.gpu
-BF16 = torch.bfloat16
+F32, F64, BF16 = torch.float32, torch.float64, torch.bfloat16
 
 
+# --------------------------------------------------------------------------------------------------- quantiser
+def nearest_codes(x):
+    """The integers nearest to 127 x / max|x|, ties to even, decided exactly: 254 |x| and an odd multiple of the maximum below 255 of it have 32 bits."""
+    x = x.to(F64)
+    top = x.abs().amax(1, keepdim=True)
+    k = torch.floor(127.0 * x.abs() / top)
+    past = 254.0 * x.abs() - (2.0 * k + 1.0) * top
+    return torch.sign(x) * torch.where((past > 0) | ((past == 0) & (k % 2 == 1)), k + 1.0, k)
+
+
+def rows_beside_borders(rows, seed):
+    """fp32 rows whose values are the nearest floats to half-integer codes, and their neighbours, of both signs, behind the row's maximum."""
+    g = gen(seed)
+    top = (1.0 + torch.rand(rows, 1, generator=g)) * torch.exp(8.0 * torch.randn(rows, 1, generator=g))
+    half = ((torch.arange(127, dtype=F64) + 0.5)[None] * top.to(F64) / 127.0).to(F32)
+    up, down = torch.nextafter(half, torch.full_like(half, math.inf)), torch.nextafter(half, torch.zeros_like(half))
+    return torch.cat([top, half, -half, up, -up, down, -down], 1)
+
+
+@pytest.mark.parametrize("copies", [1, 2, 4, 12])                             # 763 to 9156 columns: a row in one wave, in a workgroup, read twice
+def test_quant_rows_fp32_codes_beside_borders(copies):
+    x = rows_beside_borders(300, copies).repeat(1, copies)
+    x[0, :5] = torch.tensor([4.0, 2.0, -2.0, 2.0 ** -140, 0.0])               # 63.5 itself, and next to nothing
+    q, _ = K.quant_rows_i8(x.cuda())
+    assert torch.equal(q[:, :x.shape[1]].cpu().to(F64), nearest_codes(x))
+    assert torch.equal(q[0, :5].cpu()[torch.tensor([3, 4])], torch.zeros(2, dtype=torch.int8))
+
+
+def test_linear_i8_fp32_codes_beside_borders():
+    """The launch that quantises its rows itself makes the same codes."""
+    x = rows_beside_borders(40, 9).cuda()
+    k = x.shape[1]
+    w8, ws = K.quant_rows_i8(torch.randn(48, k, generator=gen(1)).cuda())
+    q = torch.zeros((40, (k + 15) // 16 * 16), dtype=torch.int8, device="cuda")
+    q[:, :k] = nearest_codes(x).to(torch.int8)
+    assert torch.equal(K.linear_i8(x, w8, ws, out_dtype=F32), K.gemm_i8(q, (x.abs().amax(1).to(F64) / 127.0).to(F32), w8, ws, out_dtype=F32))
+
+
+# --------------------------------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv_heads,q_len,cap,lens", [
     (2, 2, 4, 100, [103, 100, 101, 99, 2 ** 31 - 1, -3]),                     # the newest rows lie behind the cache; a length no cache has
