@@ -52,7 +52,7 @@ __device__ __forceinline__ float i8_relu(float x) { return x < 0.f ? 0.f : x; } 
 // addition of 1.5 2^23, whose low byte is then the code.  A bf16 x has no quotient within 2^-16 of a half that is none (2 n and an odd multiple of b are
 // multiples of 2^-14 at least); an fp32 x has, and its quotient as a float may be a half that it is not.  An element with a quotient that near a half
 // in one of the wave's rows is therefore coded again by the sign of an exact difference (quant_code_exact): about one in a thousand (4096 x 4096 in
-// fp32 14.2 us, without the second look 13.9 and 1.6e-6 of the codes wrong by one).
+// fp32 14.2 us, without the second look 13.9 and 1.2e-6 of normal rows' codes wrong by one).
 // Bound: the memory, a row is read once and held (63104 x 768 bf16 24.5 us, 6 TB/s with the codes, part of it from the last-level cache).
 struct QuantArgs { const void* x; long ldx; signed char* q; long ldq; float* scale; int M, K, Kp; };
 constexpr float kQuantTiny = 7.888609052210118e-31f;      // 2^-100
