@@ -876,6 +876,16 @@ static int gemm_i8_check(const char* who, int64_t M, int64_t N, int64_t K, const
   if (ep->aux_bf16_out && ep->ld_aux < N) return fail(ADT_EINVAL, "aux rows hold N elements");
   return ADT_OK;
 }
+// What the results may lie on.  In place every element of the residual is read and written by one lane, which needs it to be the same element in both; x: the
+// rows, in either form.
+static int gemm_i8_places_check(int64_t M, const void* x, const void* B, const void* C, int64_t ldc, const adt_gemm_epilogue* ep) {
+  if (ep->residual == C && (!ep->out_fp32 || ep->res_row_mod || (M > 1 && ep->ld_res != ldc)))
+    return set_error(ADT_EINVAL, "adt_gemm_i8: a residual in place is fp32, of C's row stride and without res_row_mod");
+  const void* aux = ep->aux_bf16_out;
+  if (C == x || C == B || (aux && (aux == x || aux == B || aux == C || aux == ep->residual)))
+    return set_error(ADT_EINVAL, "adt_gemm_i8: C and aux_bf16_out share no memory with the operands or each other");
+  return ADT_OK;
+}
 static GemmI8Args gemm_i8_args(int64_t M, int64_t N, int64_t Kp, const void* B, int64_t ldb, const float* b_scale, void* C, int64_t ldc, const adt_gemm_epilogue* ep) {
   GemmI8Args g{};
   g.B = static_cast<const signed char*>(B); g.ldb = ldb; g.b_scale = b_scale;
@@ -950,6 +960,7 @@ extern "C" int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64
   if (K & 15) return set_error(ADT_ESHAPE, "adt_gemm_i8: K must be a multiple of 16");
   if (lda < K || (lda & 15) || !aligned16(A)) return set_error(ADT_EINVAL, "adt_gemm_i8: operand rows are 16-byte aligned and hold K");
   if (M == 0 || N == 0) return ADT_OK;
+  if (int rc = gemm_i8_places_check(M, A, B, C, ldc, ep)) return rc;
   GemmI8Args g = gemm_i8_args(M, N, K, B, ldb, b_scale, C, ldc, ep);
   g.A = static_cast<const signed char*>(A); g.lda = lda; g.a_scale = a_scale;
   return ep->out_fp32 ? launch_i8<true>(g, static_cast<hipStream_t>(stream)) : launch_i8<false>(g, static_cast<hipStream_t>(stream));
@@ -975,6 +986,7 @@ extern "C" int adt_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int
   if (int rc = gemm_i8_check("adt_linear_i8", M, N, K, W, ldw, w_scale, C, ldc, ep)) return rc;
   if (ldx < K) return set_error(ADT_EINVAL, "adt_linear_i8: rows of x hold K elements");
   if (M == 0 || N == 0) return ADT_OK;
+  if (int rc = gemm_i8_places_check(M, x, W, C, ldc, ep)) return rc;
   const int64_t Kp = (K + 15) / 16 * 16;
   GemmI8Args g = gemm_i8_args(M, N, Kp, W, ldw, w_scale, C, ldc, ep);
   const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -715,7 +715,8 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
             out_dtype=torch.bfloat16, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, res_row_mod: int = 0,
             act: int = 0, aux_bf16_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act((a [M, K] @ b [N, K].T) * a_scale[:, None] * b_scale + bias) + residual`` with int8 operands and exact integer sums (``adt_gemm_i8``):
-    the inference epilogue of :func:`gemm`.  ``K`` is a multiple of 16 (``quant_rows_i8`` pads), at most 131072."""
+    the inference epilogue of :func:`gemm`.  ``K`` is a multiple of 16 (``quant_rows_i8`` pads), at most 131072.  ``residual`` may be ``out`` (fp32,
+    without ``res_row_mod``); nothing else is shared."""
     assert a.dtype == torch.int8 and b.dtype == torch.int8 and a.dim() == 2 and b.dim() == 2
     (M, K), (N, Kb), (lda, one_a), (ldb, one_b) = a.shape, b.shape, a.stride(), b.stride()
     assert K == Kb and K > 0 and K % 16 == 0 and one_a == 1 and one_b == 1, (a.shape, b.shape)
@@ -736,7 +737,7 @@ def linear_i8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, *, out: 
     """``x [M, K]`` (bf16 / fp32, row-strided views allowed) through a linear layer whose weights are int8 with one scale per output channel
     (``w8, w_scale = quant_rows_i8(weight)``): the rows are quantised (``quant_rows_i8``) and multiplied (``gemm_i8``) in one call
     (``adt_linear_i8``), small products in one launch; the same bits as the two.
-    ``out`` shares no memory with ``x``; ``residual`` may be ``out``."""
+    ``out`` and ``aux_bf16_out`` share no memory with ``x``; ``residual`` may be ``out`` (fp32, without ``res_row_mod``)."""
     assert x.dim() == 2 and w8.dim() == 2 and w8.dtype == torch.int8
     (M, K), (N, Kw), (ldx, one_x), (ldw, one_w), kind = x.shape, w8.shape, x.stride(), w8.stride(), x.dtype
     assert (kind == torch.bfloat16 or kind == torch.float32) and K > 0 and (one_x == 1 or K == 1)

@@ -470,7 +470,8 @@ int adt_gemm_bf16x3(int32_t trans, int64_t M, int64_t N, int64_t K, const void* 
  *   adt_linear_i8       both in one call: C = act(x . W^T + bias) + residual for x [M, K] bf16 / fp32 as adt_quant_rows_i8 takes it and W int8 [N, ldw],
  *                       K rounded up to 16 columns, as that leaves it.  Small products (K <= 2048) are one launch, without a workspace; the same bits either way.
  *                       ws: adt_linear_i8_workspace_bytes(M, N, K) bytes, 16-byte aligned.
- * C and aux_bf16_out share no memory with the operands; the residual may be C itself (fp32, same stride, no res_row_mod). */
+ * C and aux_bf16_out share no memory with the operands or each other; the residual may be C itself (fp32, same stride, no res_row_mod).  The same
+ * address in other roles is refused (ADT_EINVAL); a partial overlap is the caller's to avoid. */
 size_t adt_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int adt_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int32_t x_fp32, int64_t ldx, const void* W, int64_t ldw, const float* w_scale,
                   void* C, int64_t ldc, const adt_gemm_epilogue* ep, void* ws, size_t ws_bytes, void* stream);
