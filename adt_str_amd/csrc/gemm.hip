@@ -733,6 +733,12 @@ __device__ unsigned long long g_gemm_stamps[4][16][4];
 #else
 #define ADT_GSTAMP(K) do { } while (0)
 #endif
+// Epilogues that read their flags at run time (kEpiGeneric) are a few thousand instructions a piece.  Sixteen copies of that exceed what the compiler unrolls, and
+// with the strip loop left rolled the accumulators are indexed at run time: all 128 of them went through scratch (528 bytes a lane).  The strip loop is
+// unrolled here too, but the two pieces of a strip share one copy.
+__device__ __forceinline__ void read_epi_piece(unsigned at, f32x4& lo, f32x4& hi) {
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:16\n\ts_waitcnt lgkmcnt(0)" : "=&v"(lo), "=&v"(hi) : "v"(at) : "memory");
+}
 template <bool kDrop, bool kColsum, unsigned kMask, bool kX3 = false>
 __global__ __launch_bounds__(kBigThreads) void gemm_nt_256_kernel(GemmArgs g, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -942,6 +948,27 @@ __global__ __launch_bounds__(kBigThreads) void gemm_nt_256_kernel(GemmArgs g, in
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
+      auto piece = [&](int pass, const f32x4& lo, const f32x4& hi) __attribute__((always_inline)) {
+        const int row = em0 + wr * 128 + i * 16 + pass * 8 + (lane >> 3);
+        float z[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        if (row < g.M && efullL) {
+          epilogue_apply8<kDrop, kMask>(g, z, biasL, eaL, em0 + wr * 128 + (lane >> 3), i * 16 + pass * 8, ecolL);
+          if (kColsum) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) csL[e] += g.ep.out_fp32 ? z[e] : bf2f(f2bf(z[e]));
+          }
+        }
+      };
+      if constexpr ((kMask & kEpiGeneric) != 0u) {
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          f32x4 lo, hi;
+          read_epi_piece(pass ? ct_r[1] : ct_r[0], lo, hi);
+          piece(pass, lo, hi);
+        }
+        __builtin_amdgcn_wave_barrier();
+        continue;
+      }
       f32x4 zz[2][2];
       asm volatile("ds_read_b128 %0, %1" : "=v"(zz[0][0]) : "v"(ct_r[0]));
       asm volatile("ds_read_b128 %0, %1 offset:16" : "=v"(zz[0][1]) : "v"(ct_r[0]));
@@ -951,17 +978,7 @@ __global__ __launch_bounds__(kBigThreads) void gemm_nt_256_kernel(GemmArgs g, in
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_wave_barrier();                  // every lane's reads are done before the next pass overwrites the tile
 #pragma unroll
-      for (int pass = 0; pass < 2; ++pass) {
-        const int row = em0 + wr * 128 + i * 16 + pass * 8 + (lane >> 3);
-        float z[8] = {zz[pass][0][0], zz[pass][0][1], zz[pass][0][2], zz[pass][0][3], zz[pass][1][0], zz[pass][1][1], zz[pass][1][2], zz[pass][1][3]};
-        if (row < g.M && efullL) {
-          epilogue_apply8<kDrop, kMask>(g, z, biasL, eaL, em0 + wr * 128 + (lane >> 3), i * 16 + pass * 8, ecolL);
-          if (kColsum) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) csL[e] += g.ep.out_fp32 ? z[e] : bf2f(f2bf(z[e]));
-          }
-        }
-      }
+      for (int pass = 0; pass < 2; ++pass) piece(pass, zz[pass][0], zz[pass][1]);
     }
     if (kColsum) {                                      // lanes l, l + 8, ..., l + 56 hold the same 8 columns
 #pragma unroll
@@ -1637,7 +1654,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_grouped_kernel(TnGroupAr
   asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%3\n\tds_read_b64_tr_b16 %1, %2 offset:%4"            \
                : "=&v"(lo), "=&v"(hi) : "v"(addr), "i"(imm), "i"((imm) + 4096))
 
-template <bool kX3>
+template <bool kX3, unsigned kMask>
 __global__ __launch_bounds__(kBigThreads) void gemm_tn_256_kernel(GemmArgs g, int tiles_m, int tiles_n, int splits) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -1813,7 +1830,7 @@ __global__ __launch_bounds__(kBigThreads) void gemm_tn_256_kernel(GemmArgs g, in
       prologue_dma();
     }
 
-    // ---- epilogue (as gemm_nt_256_kernel): split-K items write the plain fp32 tile into their slab
+    // ---- epilogue (as gemm_nt_256_kernel): split-K items write the plain fp32 tile into their slab (kMask is kEfFp32, the weight gradients' form, for them)
     GemmArgs o = g;
     if (g.slabs) {
       o.C = g.slabs + static_cast<long>(esplit) * g.M * g.N;
@@ -1824,9 +1841,9 @@ __global__ __launch_bounds__(kBigThreads) void gemm_tn_256_kernel(GemmArgs g, in
     }
     const int ecol = en0 + wc * 64 + (lane & 7) * 8;
     const bool efull = ecol + 8 <= g.N;
-    const EpiAddr ea = epilogue_addr<false, kEpiGeneric>(o, em0 + wr * 128 + (lane >> 3), ecol);
+    const EpiAddr ea = epilogue_addr<false, kMask>(o, em0 + wr * 128 + (lane >> 3), ecol);
     float bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (o.ep.bias && efull) {            // (weight gradients carry no bias: this load is not on the hot path)
+    if ((kMask & kEpiGeneric) != 0u && o.ep.bias && efull) {
       *reinterpret_cast<float4*>(bias) = *reinterpret_cast<const float4*>(o.ep.bias + ecol);
       *reinterpret_cast<float4*>(bias + 4) = *reinterpret_cast<const float4*>(o.ep.bias + ecol + 4);
     }
@@ -1841,6 +1858,21 @@ __global__ __launch_bounds__(kBigThreads) void gemm_tn_256_kernel(GemmArgs g, in
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
+      auto piece = [&](int pass, const f32x4& lo, const f32x4& hi) __attribute__((always_inline)) {
+        const int row = em0 + wr * 128 + i * 16 + pass * 8 + (lane >> 3);
+        float z[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        if (row < g.M && efull) epilogue_apply8<false, kMask>(o, z, bias, ea, em0 + wr * 128 + (lane >> 3), i * 16 + pass * 8, ecol);
+      };
+      if constexpr ((kMask & kEpiGeneric) != 0u) {
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          f32x4 lo, hi;
+          read_epi_piece(pass ? ct_r[1] : ct_r[0], lo, hi);
+          piece(pass, lo, hi);
+        }
+        __builtin_amdgcn_wave_barrier();
+        continue;
+      }
       f32x4 zz[2][2];
       asm volatile("ds_read_b128 %0, %1" : "=v"(zz[0][0]) : "v"(ct_r[0]));
       asm volatile("ds_read_b128 %0, %1 offset:16" : "=v"(zz[0][1]) : "v"(ct_r[0]));
@@ -1850,11 +1882,7 @@ __global__ __launch_bounds__(kBigThreads) void gemm_tn_256_kernel(GemmArgs g, in
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int pass = 0; pass < 2; ++pass) {
-        const int row = em0 + wr * 128 + i * 16 + pass * 8 + (lane >> 3);
-        float z[8] = {zz[pass][0][0], zz[pass][0][1], zz[pass][0][2], zz[pass][0][3], zz[pass][1][0], zz[pass][1][1], zz[pass][1][2], zz[pass][1][3]};
-        if (row < g.M && efull) epilogue_apply8<false>(o, z, bias, ea, em0 + wr * 128 + (lane >> 3), i * 16 + pass * 8, ecol);
-      }
+      for (int pass = 0; pass < 2; ++pass) piece(pass, zz[pass][0], zz[pass][1]);
     }
     if (!more) break;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -2003,8 +2031,8 @@ static int set_big_lds_once() {      // the persistent kernels use the CU's whol
   int dev = 0;
   ADT_HIP_TRY(hipGetDevice(&dev));
   if (done_for == dev) return ADT_OK;
-  ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_tn_256_kernel<false>), hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds));
-  ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_tn_256_kernel<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds));
+  for (const auto fn : {gemm_tn_256_kernel<false, kEfFp32>, gemm_tn_256_kernel<false, kEpiGeneric>, gemm_tn_256_kernel<true, kEfFp32>, gemm_tn_256_kernel<true, kEpiGeneric>})
+    ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds));
   done_for = dev;
   return ADT_OK;
 }
@@ -2158,8 +2186,10 @@ static int gemm_bf16_impl(int32_t trans, int64_t M, int64_t N, int64_t K, const 
       for (int x = 0; x < 8; ++x)        // per slice: one ticket per work item + the ending ticket of each of its workgroups
         g.sched_total[x] = static_cast<unsigned>(items / 8 + (x < items % 8 ? 1 : 0)) + g1.x / 8 + (static_cast<unsigned>(x) < g1.x % 8 ? 1u : 0u);
       if (int rc = sched_counters(stream, &g.sched)) return rc;
-      if (g.x3_kt > 0) hipLaunchKernelGGL(gemm_tn_256_kernel<true>, g1, dim3(kBigThreads), kBigLds, st, g, tm, tn, sb);
-      else hipLaunchKernelGGL(gemm_tn_256_kernel<false>, g1, dim3(kBigThreads), kBigLds, st, g, tm, tn, sb);
+      const bool wgrad = g.slabs || epilogue_mask(e) == kEfFp32;
+      const auto fn = g.x3_kt > 0 ? (wgrad ? gemm_tn_256_kernel<true, kEfFp32> : gemm_tn_256_kernel<true, kEpiGeneric>)
+                                  : (wgrad ? gemm_tn_256_kernel<false, kEfFp32> : gemm_tn_256_kernel<false, kEpiGeneric>);
+      hipLaunchKernelGGL(fn, g1, dim3(kBigThreads), kBigLds, st, g, tm, tn, sb);
       if (sb > 1) {
         const long mn = static_cast<long>(M) * N;
         hipLaunchKernelGGL(reduce_slabs_kernel, dim3(static_cast<unsigned>((mn / 4 + 255) / 256)), dim3(256), 0, st,

@@ -58,3 +58,22 @@ def test_no_register_is_touched_with_an_lds_read_pending_and_no_packed_fp32(list
     chk = subprocess.run([sys.executable, os.path.join(ROOT, "tools", "probe", "check_pending_lds_regs.py"), str(path)], capture_output=True, text=True)
     assert chk.returncode == 0, chk.stdout[-4000:]
     assert chk.stdout.count(" 0 instruction(s)") >= min_kernels, chk.stdout[-2000:]
+
+
+def scratch_bytes(text):
+    """Kernel -> bytes of scratch per lane, from the listing's metadata."""
+    kernels = re.findall(r"^\s+\.name:\s+(\S+)$(.*?)^\s+\.private_segment_fixed_size:\s+(\d+)$", text, re.M | re.S)
+    return {name: int(size) for name, between, size in kernels if ".name:" not in between}
+
+
+def test_the_training_and_serving_kernels_keep_their_registers(listings):
+    """An accumulator array that is indexed at run time goes to memory whole: 528 bytes a lane in the 256 x 256 products, once a compiler limit kept their
+    last loop rolled.  A few dwords are spills of addresses."""
+    for name, min_kernels in SOURCES:
+        sizes = scratch_bytes(listings[name])
+        assert len(sizes) >= min_kernels, name
+        for kernel, size in sizes.items():
+            if "gemm_bf16_kernel" in kernel:                    # the fallback for operands that the others do not take
+                continue
+            most = 0 if name in ("gemm", "gemm_i8", "kv4") else 32
+            assert size <= most, (kernel, size)
