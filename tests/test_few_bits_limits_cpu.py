@@ -37,3 +37,19 @@ def test_i8_products_refuse_results_on_top_of_what_they_read(lib, linear):
     assert b"share no memory" in lib.adt_last_error()
     for at in (X, W, OUT, RES):
         assert call(aux_bf16_out=at, ld_aux=8, out_fp32=1, residual=RES, ld_res=8) == -1
+
+
+def test_linear_i8_refusals(lib):
+    need = lib.adt_linear_i8_workspace_bytes(3000, 2000, 100)
+    assert need == 3000 * 112 + 3000 * 4                                      # too many products for one launch: codes and scales
+    assert lib.adt_linear_i8_workspace_bytes(8, 8, 100) == 0 and lib.adt_linear_i8_workspace_bytes(0, 8, 100) == 0
+    big = lambda **kw: product(lib, True, **dict(dict(M=3000, N=2000, K=100, ldx=100, ldw=112, ldc=2000, ws_bytes=need), **kw))  # noqa: E731
+    assert big(ws=None) == -1 and big(ws_bytes=need - 1) == -1 and big(ws=WS + 4) == -1
+    assert b"workspace" in lib.adt_last_error()
+    for kw in (dict(x=None), dict(w=None), dict(sw=None), dict(c=None), dict(ep=False), dict(ldx=99), dict(ldw=96), dict(ldw=104), dict(w=W + 8), dict(ldc=1999), dict(act=3),
+               dict(alpha=2.0), dict(residual=RES, ld_res=1999), dict(residual=RES, ld_res=2000, res_row_mod=-1), dict(aux_bf16_out=AUX, ld_aux=2000),
+               dict(aux_bf16_out=AUX, ld_aux=1999, out_fp32=1), dict(colsum_out=RES), dict(pre_act_out=RES)):
+        assert big(**kw) == -1, kw
+    for kw in (dict(K=0), dict(K=131073, ldx=1 << 18, ldw=1 << 18), dict(M=-1), dict(N=-1), dict(M=(1 << 30) + 1)):
+        assert big(**kw) == -2, kw
+    assert big(M=0) == 0 and big(N=0, ldc=0) == 0
