@@ -907,7 +907,7 @@ static int launch_i8_tile(const GemmI8Args& g, int form, int64_t tm, int64_t tn,
   typedef void (*Fn)(GemmI8Args, int, int);
   static const Fn fns[4] = {gemm_i8_kernel<kOut32, 0, kTile, kStages>, gemm_i8_kernel<kOut32, 1, kTile, kStages>, gemm_i8_kernel<kOut32, 2, kTile, kStages>,
                             gemm_i8_kernel<kOut32, 3, kTile, kStages>};
-  if (tm * tn >= 1LL << 23) return set_error(ADT_ESHAPE, "adt_gemm_i8: too many tiles");
+  if (tm * tn >= 1LL << 24) return set_error(ADT_ESHAPE, "adt_gemm_i8: too many tiles");      // (a grid holds fewer than 2^32 threads; 2^30 x 128 results are 2^23)
   constexpr int kLds = i8_tile_lds(kTile, kStages);
   if (kLds > 65536) ADT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(fns[form]), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
   hipLaunchKernelGGL(fns[form], dim3(static_cast<unsigned>(tm * tn)), dim3(kTile == 64 ? 512 : 256), kLds, st, g, static_cast<int>(tm), static_cast<int>(tn));

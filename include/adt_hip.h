@@ -464,7 +464,7 @@ int adt_gemm_bf16x3(int32_t trans, int64_t M, int64_t N, int64_t K, const void* 
  *                       q int8 [M, ldq], columns [K, K rounded up to 16) zero; ldq a multiple of 16, rows 16-byte aligned.  A row with an
  *                       infinity or a NaN: scale NaN, codes 0, so that whatever is computed from it is NaN.
  *   adt_gemm_i8         C[M, N] = act(A[M, K] . B[N, K]^T * a_scale[m] * b_scale[n] + bias[n]) + residual, int8 operands, fp32 scales.
- *                       K a multiple of 16 up to 131072 (pad with zeros), operand rows 16-byte aligned; any M and N >= 0.
+ *                       K a multiple of 16 up to 131072 (pad with zeros), operand rows 16-byte aligned; any M and N from 0 to 2^30.
  *                       ep: bias, act, residual (+ res_row_mod), out_fp32, aux_bf16_out (with an fp32 C), as adt_gemm_bf16; alpha must be 1;
  *                       the training fields must be null / 0 (ADT_EINVAL).
  *   adt_linear_i8       both in one call: C = act(x . W^T + bias) + residual for x [M, K] bf16 / fp32 as adt_quant_rows_i8 takes it and W int8 [N, ldw],

@@ -49,6 +49,21 @@ def test_linear_i8_fp32_codes_beside_borders():
     assert torch.equal(K.linear_i8(x, w8, ws, out_dtype=F32), K.gemm_i8(q, (x.abs().amax(1).to(F64) / 127.0).to(F32), w8, ws, out_dtype=F32))
 
 
+# --------------------------------------------------------------------------------------------------- products
+def test_products_of_2_to_the_30_rows_and_of_as_many_channels():
+    """2^23 tiles, a column or a row of them; 16 GB of operands."""
+    n = 1 << 30
+    at = torch.tensor([0, 1, 127, 128, 65535, n // 2, n - 129, n - 128, n - 2, n - 1], device="cuda")
+    many, scale = torch.zeros((n, 16), dtype=torch.int8, device="cuda"), torch.ones(n, device="cuda")
+    many[at, 3] = torch.arange(1, 11, dtype=torch.int8, device="cuda")
+    scale[at] = 0.5
+    one, s1 = torch.full((1, 16), 2, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda")
+    for out in (K.gemm_i8(one, s1, many, scale)[0], K.gemm_i8(many, scale, one, s1)[:, 0]):
+        assert out[at].tolist() == [float(i) for i in range(1, 11)]
+        assert int((out != 0).sum()) == 10
+        del out
+
+
 # --------------------------------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv_heads,q_len,cap,lens", [
