@@ -78,7 +78,7 @@ __device__ unsigned long long g_fwd_stamps[32];
 // kBits (dropout only): every keep decision also goes to AttnArgs::keep_bits for the backward (attn_common.h keep_bits_*).  The compare that
 // feeds the select IS the word the backward wants (a 64-bit lane mask in a scalar register pair): its two halves are written into lanes of one
 // register (v_writelane_b32), which leaves with a block's 32 words as one 128-byte vector store.
-__device__ unsigned write_lane(unsigned value, unsigned lane, unsigned old) __asm("llvm.amdgcn.writelane.i32");      // (clang has no builtin of that name)
+__device__ unsigned write_lane(unsigned value, unsigned lane, unsigned old) __asm("llvm.amdgcn.writelane.i32");      // (clang has no builtin of that name; a compiler that does not take the label for the instruction leaves a name that nothing defines, and the library does not link)
 template <bool kDrop, int kWaves, bool kBits = false>
 __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void attn_fwd2_kernel(AttnArgs a, int n_items) {
   static_assert(kDrop || !kBits, "keep bits exist with dropout only");

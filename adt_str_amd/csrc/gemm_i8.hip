@@ -27,8 +27,9 @@ __device__ __forceinline__ unsigned i8_pack_bf2(float lo, float hi) {
 }
 
 // GELU(x) = max(x, 0) - |x| Q(|x|), Q(a) = erfc(a / sqrt 2) / 2 = 2^P8(a): a polynomial fitted to log2 Q with Q as the weight, so that the error of |x| Q is
-// 4e-8 at most, fp32 rounding included, and for every a (the leading coefficient is negative: past the fit's 5.5, where Q is 2e-8, 2^P8 falls faster
-// than Q).  One v_exp and eleven plain instructions on scalars, as packed fp32 ones are off; with erfc as t P5(t) exp(-a^2 / 2), t = 1 / (1 + c a), 63104 x 2304
+// 4.1e-8 at most (at 1.54), fp32 rounding included, 4.8e-8 with an exponential that is off by its last place, and for every a (the leading coefficient is
+// negative: past the fit's 5.5, where Q is 2e-8, 2^P8 falls faster than Q).  Relative to the tail itself that is 1 % at -5, 12 % at -6, 56 % at -7, where
+// GELU is -1.4e-6, -6e-9 and -9e-12.  One v_exp and eleven plain instructions on scalars, as packed fp32 ones are off; with erfc as t P5(t) exp(-a^2 / 2), t = 1 / (1 + c a), 63104 x 2304
 // x 768 took 178 us, with this 170.  (The factor is held below infinity: infinity times zero is no number.)
 __device__ __forceinline__ float i8_gelu(float x) {
   const float a = fabsf(x);

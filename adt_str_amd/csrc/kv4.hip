@@ -2,7 +2,8 @@
 //
 // Every 64 channels of a K or V row (one token, one head) share a scale and a minimum:
 //   lo = min x, hi = max x, s = bf16(max((hi - lo) / 15, 2^-100)), m = lo, c = the integer nearest to (x - lo) / s (ties to even, at most 15)
-//   and the row stands for c s + m.  A group with an infinity or a NaN (or a range past fp32): s = m = NaN.
+//   and the row stands for c s + m.  A group with an infinity or a NaN (or a range past fp32): s = m = NaN.  The differences are fp32's: exact unless two
+//   values of the group are more than 2^16 apart; the quotients of them are decided as real numbers are.
 //
 // Layout: per (sequence, head) a run of tiles of 32 tokens, per tile of head_dim D one record
 //   K codes 32 D / 2 | V codes 32 D / 2 | K parameters [D/64][32] | V parameters [D/64][32]        4608 bytes at D = 128 (16384 in bf16)
@@ -642,7 +643,9 @@ static int kv_rows_check(const char* who, int64_t B, int64_t H, int64_t D, const
 struct KvPlan { int rows, row_blocks, tiles, spans, span_tiles, waves; };
 // How a call is cut.  A wave's tile costs 1 us when it has its SIMD to itself (420 instructions), a call 5 us around its tiles and 2 us more for the
 // join of spans.  A workgroup of eight waves fills half a CU or more, of four a third.  us with waves / spans, heads x positions:
-//   at most one workgroup a CU and three tiles a wave: eight waves, one span (16 x 582 8/1 5.3, 4/1 5.4, 4/6 7.5);
+//   at most one workgroup a CU and 26 tiles, three a wave and a fourth in two of them: eight waves, one span.  The border is a compromise between few and many
+//   heads (one query, 128 channels; 6 heads x 24 tiles 8/1 8.0, 4/4 7.7, 4/8 7.0, 27 tiles 8.5, 7.8, 6.9; 192 heads x 24 tiles 8/1 8.3, 4/2 10.7, 4/4
+//   10.6, 27 tiles 8.9, 12.3, 11.2: one span is as good or better to 20 tiles everywhere, and to 34 for 192 heads);
 //   one to four rows: four waves, and spans until the card is full, or of 32 tiles, as short sequences leave theirs empty and the late
 //   ones even that out (6 x 986 4/8 7.3, 8/4 8.3, 8/1 9.6; 64 x 32000 in four rows, ragged, 4/24 39, 4/12 53, 8/4 55; 174 x 21483 4/24 41, 4/4 59, 8/2 74);
 //   more rows, whose joins weigh more: eight waves, spans for one workgroup a CU, or of 64 tiles (60 x 2359 in 16 rows 8/4 13.6, 4/12 15.1; 108 x 4271

@@ -485,7 +485,8 @@ int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, con
  * The caches of the KV-cached greedy decode (reference model.py:260-324 re-runs the decoder instead) at 72 bytes per K or V row of 128
  * channels instead of 256.  Every 64 channels of a row share a bf16 scale s and a bf16 minimum m; a value is c s + m with a code c in 0 .. 15:
  *   m = min x,  s = bf16(max((max x - m) / 15, 2^-100)),  c = min(15, the integer nearest to (x - m) / s, ties to even)
- * A group with an infinity or a NaN, or whose range exceeds fp32, stands for NaNs.
+ * A group with an infinity or a NaN, or whose range exceeds fp32, stands for NaNs.  The differences are formed in fp32, which is exact unless two
+ * values of a group are more than 2^16 apart.
  *
  *   adt_kv4_bytes    size of a cache of `capacity` positions per sequence (head_dim 64 or 128); opaque device memory, 16-byte aligned.  It
  *                    need not be cleared: only rows below the lengths that a call names are read.  Calls on one cache follow one another (one
@@ -498,7 +499,9 @@ int adt_gemm_i8(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, con
  *                    head_dim].  heads is a multiple of kv_heads: query heads g * kv_head .. + g - 1 read K/V head kv_head (g = heads / kv_heads).
  *                    causal: query i sees the positions below key_len[b] - (q_len - 1 - i), that is, the queries are the sequence's last
  *                    positions.  Of a sequence that is longer than the capacity the cache has the first `capacity` positions, and a query sees
- *                    those of its own that are among them.  A query that sees no position gets zeros (lse -inf).  lse: optional fp32 [batch, heads, q_len]. */
+ *                    those of its own that are among them.  A query that sees no position gets zeros (lse -inf).  lse: optional fp32 [batch, heads, q_len].
+ *                    At most 2^24 query rows (q_len * g) per K/V head and 2^23 workgroups of 16 rows and a span (ADT_ESHAPE); every 16 rows read the cache.
+ * Caches have at most 65535 sequences and heads and 2^30 positions (ADT_ESHAPE). */
 size_t adt_kv4_bytes(int64_t batch, int32_t kv_heads, int32_t head_dim, int64_t capacity);
 int adt_kv4_append(void* cache, int64_t batch, int32_t kv_heads, int32_t head_dim, int64_t capacity, const void* k, int64_t ldk, const void* v,
                    int64_t ldv, int64_t n, const int32_t* end, const int32_t* count, void* stream);
