@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from adt_str_amd import kernels as K
-from tests.test_few_bits_gpu import check_attn, check_held, gen, kv_rows
+from tests.test_few_bits_gpu import attn_ref, check_attn, check_held, gen, kv_rows
 
 pytestmark = pytest.mark.gpu
 F32, F64, BF16 = torch.float32, torch.float64, torch.bfloat16
@@ -99,3 +99,66 @@ def test_append_and_causal_attention_of_a_sequence_that_outgrows_its_cache():
     q = torch.randn(q_len, heads * dim, generator=gen(9)).to(BF16).cuda()
     out, lse = K.attn_kv4(q, c, at(end), heads=heads, scale=dim ** -0.5, q_len=q_len, causal=True, want_lse=True)
     check_attn(out, lse, q, k[None, :cap], v[None, :cap], heads, heads, dim, 1, q_len, [end], dim ** -0.5, True)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 20.0, -20.0])
+@pytest.mark.parametrize("heads,kv_heads,q_len,cap,lens", [(3, 3, 1, 90, [90, 33, 0]), (6, 2, 5, 200, [200, 3, 64]), (2, 1, 1, 2500, [2500, 1, 999])])
+def test_attn_kv4_scales_of_any_sign_and_size(dim, scale, heads, kv_heads, q_len, cap, lens):
+    batch = len(lens)
+    k, v = kv_rows(batch * cap, kv_heads, dim, cap)
+    c = K.KV4Cache(batch, cap, kv_heads, dim)
+    K.kv4_append(c, k, v)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch * q_len, heads * dim, generator=gen(2)).to(BF16).cuda()
+    out, lse = K.attn_kv4(q, c, n, heads=heads, scale=scale, q_len=q_len, causal=True, want_lse=True)
+    q_ref = -q if scale < 0 else q                                            # exact: a negative scale is the negative query's
+    o, l, mag = attn_ref(q_ref, k.reshape(batch, cap, -1), v.reshape(batch, cap, -1), heads, kv_heads, dim, batch, q_len, lens, abs(scale), True)
+    assert ((out.to(F64) - o).abs() <= 2.0 ** -8 * (o.abs() + mag) + mag).all()
+    none = l == -math.inf
+    assert torch.equal(lse == -math.inf, none)
+    # the score's own error (8 roundings of about 31 steps of 0.4 and 1.5 against each of dim unit query values), times the scale, and two of the log-sum's
+    dz = 8 * 2.0 ** -24 * 14.0 * dim * abs(scale)
+    assert ((lse.to(F64) - l)[~none].abs() <= dz + 2.0 ** -23 * l[~none].abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap", [70, 3000])                                   # one span, several
+def test_attn_kv4_query_rows_without_numbers_stay_alone(dim, cap):
+    heads, kv_heads, q_len = 4, 2, 6
+    k, v = kv_rows(2 * cap, kv_heads, dim, 8)
+    c = K.KV4Cache(2, cap, kv_heads, dim)
+    K.kv4_append(c, k, v)
+    q = torch.randn(2 * q_len, heads * dim, generator=gen(3)).to(BF16).cuda()
+    clean = K.attn_kv4(q, c, heads=heads, scale=0.1, q_len=q_len).reshape(2 * q_len, heads, dim)
+    q[3, 2 * dim + 5] = math.nan                                              # row 3, head 2
+    q[7, 1] = math.inf                                                        # row 7, head 0
+    out = K.attn_kv4(q, c, heads=heads, scale=0.1, q_len=q_len).reshape(2 * q_len, heads, dim)
+    bad = torch.zeros(2 * q_len, heads, dtype=torch.bool, device="cuda")
+    bad[3, 2] = bad[7, 0] = True
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_kv4_append_rows_that_begin_anywhere_and_more_of_them_than_positions(dim):
+    batch, heads, cap, n = 2, 3, 37, 90
+    width = heads * dim
+    g = gen(11)
+    kb, vb = torch.randn(batch * n, width + 3, generator=g).to(BF16).cuda(), torch.randn(batch * n, width + 16, generator=g).to(BF16).cuda()
+    k, v = kb[:, 1:1 + width], vb[:, 8:8 + width]                             # keys two bytes at a time, values sixteen
+    for a, b in ((k, v), (v, k)):
+        c = K.KV4Cache(batch, cap, heads, dim)
+        c.data.fill_(0xFF)
+        K.kv4_append(c, a, b)                                                 # n rows for cap positions: the last ones
+        held = K.kv4_read(c, out_dtype=F32)
+        for got, src in zip(held, (a, b)):
+            check_held(got, src.reshape(batch, n, width)[:, n - cap:].reshape(batch * cap, width), heads, dim)
+        end = torch.tensor([60, 5], dtype=torch.int32, device="cuda")         # sequence 0: rows 30 .. 66 of 90 fit, 1: its last five
+        c.data.fill_(0xFF)
+        K.kv4_append(c, a, b, end)
+        back = K.kv4_read(c, end, None, n, out_dtype=F32)
+        for got, src in zip(back, (a, b)):
+            got, src = got.reshape(batch, n, width), src.reshape(batch, n, width)
+            check_held(got[0, 30:67], src[0, 30:67], heads, dim)
+            check_held(got[1, 85:], src[1, 85:], heads, dim)
+            assert not got[0, :30].any() and not got[0, 67:].any() and not got[1, :85].any()
