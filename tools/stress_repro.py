@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Race hunt (GPU box): the kernels are deterministic, so any run-to-run difference of the outputs of the hand-synchronised kernels
-(attention forward / backward at the encoder and decoder shapes, persistent NT / TN GEMMs in the step's forms, the fused HTSAT
-tower) is a synchronisation bug.
+(attention forward / backward at the encoder and decoder shapes, persistent NT / TN GEMMs in the step's forms, the 8-bit-integer products and the
+4-bit cache, the fused HTSAT tower) is a synchronisation bug.
 Usage: python tools/stress_repro.py [iterations]"""
 import math
 import os
@@ -81,6 +81,28 @@ b2 = torch.randn(768, device=dev)
 check("NT 256^2 FFN2 + bias + dropout + residual (fp32 out)", lambda: (K.gemm(x, w2, bias=b2, residual=res, out_dtype=torch.float32, drop=(0.1, 11)),))
 wq = torch.randn((2304, 768), device=dev).bfloat16()
 check("NT 256^2 QKV (column-group tile order, 9 tile columns)", lambda: (K.gemm(a, wq, bias=torch.zeros(2304, device=dev)),))
+
+resq, copyq = torch.randn((M, 2304), device=dev), torch.empty((M, 2304), dtype=torch.bfloat16, device=dev)
+check("NT 256^2 with flags read at run time (bias, ReLU, residual, copy)", lambda: (K.gemm(a, wq, bias=torch.zeros(2304, device=dev), act=2, out_dtype=torch.float32,
+                                                                                         residual=resq, aux_bf16_out=copyq), copyq))
+# 8-bit products: two or three 256 x 256 tiles a workgroup, each output type and epilogue; the other tile sizes
+for (m, n, k) in [(M, 2304, 768), (20001, 2301, 384), (7747, 768, 768), (1000, 1000, 4800), (300, 701, 400), (64, 1400, 768)]:
+    xi = torch.randn((m, k), device=dev).bfloat16()
+    wi, si = K.quant_rows_i8(torch.randn((n, k), device=dev))
+    bi, ri = torch.randn(n, device=dev), torch.randn((m, n), device=dev)
+    check(f"int8 {m} x {n} x {k}, bias", lambda: (K.linear_i8(xi, wi, si, bias=bi),))
+    check(f"int8 {m} x {n} x {k}, GELU", lambda: (K.linear_i8(xi, wi, si, bias=bi, act=1),))
+    check(f"int8 {m} x {n} x {k}, fp32, residual", lambda: (K.linear_i8(xi, wi, si, bias=bi, residual=ri, out_dtype=torch.float32),))
+for (B, kv_heads, heads, dim, keys, q_len) in [(1, 6, 6, 128, 986, 1), (64, 6, 6, 128, 986, 1), (8, 8, 32, 128, 32000, 1), (24, 5, 10, 64, 3001, 7)]:
+    rows = torch.randn((B * keys, 2 * kv_heads * dim), device=dev).bfloat16()
+    qi = torch.randn((B * q_len, heads * dim), device=dev).bfloat16()
+    cache = K.KV4Cache(B, keys, kv_heads, dim, dev)
+
+    def cached():
+        K.kv4_append(cache, rows[:, :kv_heads * dim], rows[:, kv_heads * dim:])
+        return K.kv4_read(cache, n=min(keys, 1000)) + K.attn_kv4(qi, cache, heads=heads, scale=dim ** -0.5, q_len=q_len, causal=q_len > 1, want_lse=True)
+
+    check(f"4-bit cache {B} x {kv_heads}/{heads} x {keys}, {q_len} queries: append, read, attention", cached)
 
 # the split-bf16 parity arm's large products on the persistent kernels (round 6: virtual-K-tile operand map, planes split once)
 K.set_f32_products("bf16x3")
